@@ -345,6 +345,20 @@ int madiff_adam_ema(float* p, float* g, float* m, float* v, float* ema, long n, 
                     float eps, float bc1, float bc2_sqrt, float grad_scale, int do_ema, float ema_beta, int* state,
                     void* shadow_bf16, int zero_grad, madiff_stream_t stream);
 
+/* Layer norm over the first C columns of every row (no counterpart selected by the reference's configurations: its
+ * denoiser takes use_layer_norm, models/ma_temporal.py:245):  y = (x - mean) * rstd * w + b, rstd = (var + eps)^-1/2.
+ * x, y [rows, ld] in `dtype`, any element-aligned row address; w, b fp32 [C] or NULL (1 and 0); mean, rstd fp32 [rows], both or
+ * neither (backward needs them).  Columns [C, Cpad) of y are written as zeros.  1 <= C <= 32768. */
+int madiff_layer_norm_fwd(int dtype, const void* x, long ldx, void* y, long ldy, const float* w, const float* b, float* mean,
+                          float* rstd, long rows, int C, int Cpad, float eps, madiff_stream_t stream);
+/* Its gradients: dx (NULL: not wanted; columns [C, Cpad) zeroed) and dw, db (NULL: not wanted), which are overwritten, or added
+ * to where accumulate != 0.  ws: 2 * C * madiff_layer_norm_groups(dtype, rows, C) floats, only read behind this call's own
+ * writes, needed for dw / db.  The same call gives the same bits (no atomics). */
+int madiff_layer_norm_groups(int dtype, long rows, int C);
+int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, long lddy, const float* w, const float* mean,
+                          const float* rstd, void* dx, long lddx, float* dw, float* db, int accumulate, float* ws,
+                          long ws_floats, long rows, int C, int Cpad, madiff_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

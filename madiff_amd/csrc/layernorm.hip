@@ -1,0 +1,410 @@
+// Layer norm over the channels of channels-last rows, forward and backward.
+//
+//   mu = mean_c x,  v = mean_c (x - mu)^2,  r = (v + eps)^-1/2,  h = (x - mu) r,  y = h w + b
+//   g = dy w,  dx = r (g - mean_c g - h mean_c(g h)),  dw = sum_rows dy h,  db = sum_rows dy
+//
+// Bandwidth-bound: forward reads x and writes y once, backward reads x and dy and writes dx once.  A row lives in the
+// registers of a group of lanes: 8..64 lanes of one wave while R <= 4 vectors of 16 bytes a lane hold it, else a
+// workgroup of 256 or 1024 lanes.  Groups stride over the rows with their share of w and b in registers (read from L2
+// for every row they would cost four times the bf16 row itself) and with the next row's loads in flight.  The variance
+// is the second pass over the registers, not E[x^2] - mu^2.  All arithmetic is fp32; the only rounding to fewer bits is
+// that of y and dx to the storage type of x.
+// dw / db: every lane sums its own columns over the rows of its group in fp32 registers, a workgroup's groups meet in LDS,
+// each workgroup leaves one [2, C] partial, and a second launch adds the partials in index order: no atomics, so the same
+// call gives the same bits.
+#include "common.h"
+
+template <typename T> struct LnVec { static constexpr int N = 16 / sizeof(T); T v[N]; };
+
+// 16 bytes from an address that is only element-aligned (rows of odd widths begin anywhere; the hardware takes it)
+template <typename T> __device__ __forceinline__ LnVec<T> ln_load(const T* p) {
+  LnVec<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T> __device__ __forceinline__ LnVec<T> ln_load_part(const T* p, int n) {   // n elements, zeros behind
+  LnVec<T> r;
+#pragma unroll
+  for (int e = 0; e < LnVec<T>::N; e++) r.v[e] = e < n ? p[e] : from_f32<T>(0.f);
+  return r;
+}
+// one lane's R vectors of a row: columns (l + i LPR) N .. + N
+template <typename T, int LPR, int R>
+__device__ __forceinline__ void ln_row(LnVec<T> (&d)[R], const T* row, int l, int C) {
+  constexpr int N = LnVec<T>::N;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int c = (l + i * LPR) * N;
+    if (c + N <= C) d[i] = ln_load(row + c);
+    else d[i] = ln_load_part(row + (c < C ? c : 0), c < C ? C - c : 0);
+  }
+}
+// N gains (or shifts) from column c on; `none` where there is no such vector, 0 behind the row's end
+template <int N>
+__device__ __forceinline__ void ln_gain(float (&d)[N], const float* w, int c, int C, float none) {
+  if (w && c + N <= C) {
+    __builtin_memcpy(d, w + c, 4 * N);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e++) d[e] = c + e < C ? (w ? w[c + e] : none) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void ln_put(T* row, const float (&y)[LnVec<T>::N], int c, int C) {
+  constexpr int N = LnVec<T>::N;
+  if (c + N <= C) {
+    LnVec<T> o;
+#pragma unroll
+    for (int e = 0; e < N; e++) o.v[e] = from_f32<T>(y[e]);
+    __builtin_memcpy(row + c, &o, 16);
+  } else if (c < C) {
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (c + e < C) row[c + e] = from_f32<T>(y[e]);
+  }
+}
+
+// Sum of K values over the LPR lanes of a group.  Within a wave by shuffles; across the waves of a workgroup through LDS,
+// in wave order.  `slot` alternates from call to call, so that one barrier a call is enough: the values of a call are
+// overwritten two calls later, behind the barrier of the call between.
+template <int LPR, int K>
+__device__ __forceinline__ void ln_sum(float (&v)[K], float* lds, int& slot) {
+#pragma unroll
+  for (int k = 0; k < K; k++)
+#pragma unroll
+    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
+  if constexpr (LPR > 64) {
+    constexpr int W = LPR / 64;
+    float* s = lds + slot * (K * W);
+    slot ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < K; k++) s[k * W + (threadIdx.x >> 6)] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; w++) v[k] += s[k * W + w];
+    }
+  }
+}
+
+template <typename T, int LPR, int R>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
+    const T* __restrict__ x, long ldx, T* __restrict__ y, long ldy, const float* __restrict__ w, const float* __restrict__ b,
+    float* __restrict__ mean_out, float* __restrict__ rstd_out, long rows, int C, int Cpad, float eps) {
+  constexpr int N = LnVec<T>::N, BLOCK = LPR > 256 ? LPR : 256, GPB = LPR > 64 ? 1 : BLOCK / LPR;
+  __shared__ float lds[LPR > 64 ? 2 * (LPR / 64) : 1];
+  const int l = threadIdx.x % LPR;
+  const long g0 = (long)blockIdx.x * GPB + (GPB > 1 ? threadIdx.x / LPR : 0), gs = (long)gridDim.x * GPB;
+  int slot = 0;
+  constexpr bool LEAN = LPR == 1024;     // 128 registers a lane: gains and shifts come from L2 row by row, no row is prefetched
+  float wv[LEAN ? 1 : R][N], bv[LEAN ? 1 : R][N];
+  if constexpr (!LEAN)
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      ln_gain<N>(wv[i], w, (l + i * LPR) * N, C, 1.f);
+      ln_gain<N>(bv[i], b, (l + i * LPR) * N, C, 0.f);
+    }
+  LnVec<T> nx[R];
+  if (!LEAN && g0 < rows) ln_row<T, LPR, R>(nx, x + g0 * ldx, l, C);
+  const float inv = 1.f / (float)C;
+  for (long r = g0; r < rows; r += gs) {
+    const float *wr = w, *br = b;
+    if constexpr (LEAN) {
+      asm("" : "+s"(wr), "+s"(br));        // (not loop-invariant to the compiler: it would hold them in registers)
+      ln_row<T, LPR, R>(nx, x + r * ldx, l, C);
+    }
+    float v[R][N];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        v[i][e] = to_f32(nx[i].v[e]);
+        s[0] += v[i][e];
+      }
+    if (!LEAN && r + gs < rows) ln_row<T, LPR, R>(nx, x + (r + gs) * ldx, l, C);
+    ln_sum<LPR, 1>(s, lds, slot);
+    const float mean = s[0] / (float)C;      // (divided: the mean of equal values is that value)
+    s[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        v[i][e] -= mean;
+        const float d = (l + i * LPR) * N + e < C ? v[i][e] : 0.f;
+        s[0] += d * d;
+      }
+    ln_sum<LPR, 1>(s, lds, slot);
+    const float rstd = 1.f / sqrtf(s[0] * inv + eps);
+    if (l == 0 && mean_out) { mean_out[r] = mean; rstd_out[r] = rstd; }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      if constexpr (LEAN) {
+        ln_gain<N>(wv[0], wr, (l + i * LPR) * N, C, 1.f);
+        ln_gain<N>(bv[0], br, (l + i * LPR) * N, C, 0.f);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int e = 0; e < N; e++) v[i][e] = v[i][e] * rstd * wv[LEAN ? 0 : i][e] + bv[LEAN ? 0 : i][e];
+      ln_put<T>(y + r * ldy, v[i], (l + i * LPR) * N, C);
+    }
+    for (int c = C + l; c < Cpad; c += LPR) y[r * ldy + c] = from_f32<T>(0.f);   // pad columns of the layout stay zero
+  }
+}
+
+// part: [gridDim.x, 2, C] column sums (dw then db) of the workgroup's rows; null = no parameter gradient wanted.
+template <typename T, int LPR, int R>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
+    const T* __restrict__ x, long ldx, const T* __restrict__ dy, long lddy, const float* __restrict__ w,
+    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, long lddx,
+    float* __restrict__ part, long rows, int C, int Cpad) {
+  constexpr int N = LnVec<T>::N, BLOCK = LPR > 256 ? LPR : 256, GPB = LPR > 64 ? 1 : BLOCK / LPR;
+  constexpr int COLS = 64 * R * N;                           // columns a wave covers (LPR <= 64)
+  __shared__ float lds[LPR > 64 ? 4 * (LPR / 64) : 3 * COLS];
+  const int l = threadIdx.x % LPR;
+  const long g0 = (long)blockIdx.x * GPB + (GPB > 1 ? threadIdx.x / LPR : 0), gs = (long)gridDim.x * GPB;
+  int slot = 0;
+  constexpr bool LEAN = LPR == 1024;     // 128 registers a lane: the row stays in its storage type, h and g are formed twice
+  float wv[LEAN ? 1 : R][N], aw[R][N], ab[R][N];
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    if constexpr (!LEAN) ln_gain<N>(wv[i], w, (l + i * LPR) * N, C, 1.f);
+#pragma unroll
+    for (int e = 0; e < N; e++) aw[i][e] = ab[i][e] = 0.f;
+  }
+  LnVec<T> nx[R], nd[R];
+  if (!LEAN && g0 < rows) {
+    ln_row<T, LPR, R>(nx, x + g0 * ldx, l, C);
+    ln_row<T, LPR, R>(nd, dy + g0 * lddy, l, C);
+  }
+  const float inv = 1.f / (float)C;
+  for (long r = g0; r < rows; r += gs) {
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    const float* wr = w;
+    if constexpr (LEAN) {
+      asm("" : "+s"(wr));
+      ln_row<T, LPR, R>(nx, x + r * ldx, l, C);
+      ln_row<T, LPR, R>(nd, dy + r * lddy, l, C);
+    }
+    float h[LEAN ? 1 : R][N], g[LEAN ? 1 : R][N];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int k = LEAN ? 0 : i;
+      if constexpr (LEAN) {
+        ln_gain<N>(wv[0], wr, (l + i * LPR) * N, C, 1.f);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const float d = to_f32(nd[i].v[e]);                  // 0 behind the row's end, and so is all it multiplies
+        h[k][e] = (to_f32(nx[i].v[e]) - mean) * rstd;
+        g[k][e] = d * wv[k][e];
+        aw[i][e] += d * h[k][e];
+        ab[i][e] += d;
+        s[0] += g[k][e];
+        s[1] += g[k][e] * h[k][e];
+      }
+    }
+    if (!LEAN && r + gs < rows) {
+      ln_row<T, LPR, R>(nx, x + (r + gs) * ldx, l, C);
+      ln_row<T, LPR, R>(nd, dy + (r + gs) * lddy, l, C);
+    }
+    if (dx) {
+      ln_sum<LPR, 2>(s, lds, slot);
+      const float c1 = s[0] * inv, c2 = s[1] * inv;
+      if constexpr (LEAN) asm("" : "+s"(wr));
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int k = LEAN ? 0 : i;
+        if constexpr (LEAN) {
+
+          ln_gain<N>(wv[0], wr, (l + i * LPR) * N, C, 1.f);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = 0; e < N; e++) {
+            h[0][e] = (to_f32(nx[i].v[e]) - mean) * rstd;
+            g[0][e] = to_f32(nd[i].v[e]) * wv[0][e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) g[k][e] = rstd * (g[k][e] - c1 - h[k][e] * c2);
+        ln_put<T>(dx + r * lddx, g[k], (l + i * LPR) * N, C);
+      }
+      for (int c = C + l; c < Cpad; c += LPR) dx[r * lddx + c] = from_f32<T>(0.f);
+    }
+  }
+  if (!part) return;
+  float* out = part + (size_t)blockIdx.x * 2 * C;
+  if constexpr (LPR > 64) {                                  // every lane owns its columns
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const int c = (l + i * LPR) * N + e;
+        if (c < C) { out[c] = aw[i][e]; out[C + c] = ab[i][e]; }
+      }
+  } else {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int q = 0; q < 2; q++) {                            // the groups of a wave, then the four waves in order
+#pragma unroll
+      for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          float a = q ? ab[i][e] : aw[i][e];
+#pragma unroll
+          for (int o = LPR; o < 64; o <<= 1) a += __shfl_xor(a, o, 64);
+          if (q) ab[i][e] = a; else aw[i][e] = a;
+        }
+      __syncthreads();
+      if (wave > 0 && lane < LPR)
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+          for (int e = 0; e < N; e++) lds[(wave - 1) * COLS + (i * N + e) * LPR + l] = q ? ab[i][e] : aw[i][e];
+      __syncthreads();
+      if (wave == 0 && lane < LPR)
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+          for (int e = 0; e < N; e++) {
+            float a = q ? ab[i][e] : aw[i][e];
+#pragma unroll
+            for (int o = 0; o < 3; o++) a += lds[o * COLS + (i * N + e) * LPR + l];
+            const int c = (l + i * LPR) * N + e;
+            if (c < C) out[q * C + c] = a;
+          }
+    }
+  }
+}
+
+// dw / db (+)= sum over the partials, in index order: 64 columns a workgroup, 16 lanes a column.
+__global__ __launch_bounds__(1024) void layer_norm_param_kernel(const float* __restrict__ part, int n, int C,
+                                                               float* __restrict__ dw, float* __restrict__ db, int accumulate) {
+  __shared__ float lds[16][64];
+  const int cl = threadIdx.x & 63, k = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + cl;                        // column of [2, C]
+  float s = 0.f;
+  if (c < 2 * C) {
+    const int per = (n + 15) / 16, lo = k * per, hi = min(n, lo + per);
+    const float* p = part + (size_t)lo * 2 * C + c;
+#pragma unroll 8
+    for (int i = lo; i < hi; i++, p += 2 * (size_t)C) s += *p;
+  }
+  lds[k][cl] = s;
+  __syncthreads();
+  if (k == 0 && c < 2 * C) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s += lds[i][cl];
+    float* o = c < C ? (dw ? dw + c : nullptr) : (db ? db + (c - C) : nullptr);
+    if (o) *o = accumulate ? *o + s : s;
+  }
+}
+
+#define LN_MAX_COLS 32768
+
+static inline int ln_groups_per_block(int dtype, int C) {    // rows a workgroup works on at once
+  const int n = dtype == MADIFF_BF16 ? 8 : 4, v = (C + n - 1) / n;
+  if (v > 256) return 1;
+  int lpr = 8;
+  while (lpr < v && lpr < 64) lpr <<= 1;
+  return 256 / lpr;
+}
+static inline long ln_blocks(int dtype, long rows, int C, int per_group, int most) {
+  const long gpb = ln_groups_per_block(dtype, C);
+  const long b = (rows + gpb * per_group - 1) / (gpb * per_group);
+  return b < 1 ? 1 : (b > most ? most : b);
+}
+
+// calls F<T, LPR, R> for the row width; the widths that R = 1 .. 4 vectors of one wave hold stay in one wave
+#define LN_DISPATCH(F)                                                   \
+  do {                                                                   \
+    constexpr int N = 16 / sizeof(T);                                    \
+    const int v = (C + N - 1) / N;                                       \
+    if (v <= 8) F(8, 1);                                                 \
+    else if (v <= 16) F(16, 1);                                          \
+    else if (v <= 32) F(32, 1);                                          \
+    else if (v <= 64) F(64, 1);                                          \
+    else if (v <= 128) F(64, 2);                                         \
+    else if (v <= 192) F(64, 3);                                         \
+    else if (v <= 256) F(64, 4);                                         \
+    else if (v <= 512) F(256, 2);                                        \
+    else if (v <= 1024) F(256, 4);                                       \
+    else if (v <= 2048) F(1024, 2);                                      \
+    else if (v <= 4096) F(1024, 4);                                      \
+    else if constexpr (N == 4) F(1024, 8);                               \
+  } while (0)
+
+template <typename T>
+static int ln_fwd(const T* x, long ldx, T* y, long ldy, const float* w, const float* b, float* mean, float* rstd, long rows,
+                  int C, int Cpad, float eps, hipStream_t st) {
+  const int dt = sizeof(T) == 2 ? MADIFF_BF16 : MADIFF_F32;
+  const dim3 grid((unsigned)ln_blocks(dt, rows, C, 1, 2048));
+#define LN_F(LPR, R)                                                                                                      \
+  hipLaunchKernelGGL((layer_norm_fwd_kernel<T, LPR, R>), grid, dim3(LPR > 256 ? LPR : 256), 0, st, x, ldx, y, ldy, w, b, \
+                     mean, rstd, rows, C, Cpad, eps)
+  LN_DISPATCH(LN_F);
+#undef LN_F
+  MADIFF_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T>
+static int ln_bwd(const T* x, long ldx, const T* dy, long lddy, const float* w, const float* mean, const float* rstd, T* dx,
+                  long lddx, float* part, int groups, long rows, int C, int Cpad, hipStream_t st) {
+#define LN_B(LPR, R)                                                                                                      \
+  hipLaunchKernelGGL((layer_norm_bwd_kernel<T, LPR, R>), dim3(groups), dim3(LPR > 256 ? LPR : 256), 0, st, x, ldx, dy,   \
+                     lddy, w, mean, rstd, dx, lddx, part, rows, C, Cpad)
+  LN_DISPATCH(LN_B);
+#undef LN_B
+  MADIFF_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int madiff_layer_norm_fwd(int dtype, const void* x, long ldx, void* y, long ldy, const float* w, const float* b,
+                                     float* mean, float* rstd, long rows, int C, int Cpad, float eps, hipStream_t stream) {
+  if ((dtype != MADIFF_F32 && dtype != MADIFF_BF16) || rows < 0 || C < 1 || C > LN_MAX_COLS || Cpad < C || ldx < C ||
+      ldy < Cpad || !(eps >= 0.f) || (mean == nullptr) != (rstd == nullptr))
+    return -1;
+  if (rows == 0) return 0;
+  if (!x || !y) return -1;
+  return dtype == MADIFF_BF16
+             ? ln_fwd<bf16_t>((const bf16_t*)x, ldx, (bf16_t*)y, ldy, w, b, mean, rstd, rows, C, Cpad, eps, stream)
+             : ln_fwd<float>((const float*)x, ldx, (float*)y, ldy, w, b, mean, rstd, rows, C, Cpad, eps, stream);
+}
+
+extern "C" int madiff_layer_norm_groups(int dtype, long rows, int C) {
+  if ((dtype != MADIFF_F32 && dtype != MADIFF_BF16) || rows < 0 || C < 1 || C > LN_MAX_COLS) return -1;
+  return (int)ln_blocks(dtype, rows, C, 4, C > 2048 ? 256 : 1024);
+}
+
+extern "C" int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, long lddy, const float* w,
+                                     const float* mean, const float* rstd, void* dx, long lddx, float* dw, float* db,
+                                     int accumulate, float* ws, long ws_floats, long rows, int C, int Cpad,
+                                     hipStream_t stream) {
+  const int groups = madiff_layer_norm_groups(dtype, rows, C);
+  const bool params = dw || db;
+  if (groups < 0 || Cpad < C || ldx < C || lddy < C || (dx && lddx < Cpad) || (params && (!ws || ws_floats < 2L * groups * C)))
+    return -1;
+  if (rows > 0) {
+    if (!x || !dy || !mean || !rstd) return -1;
+    if (!dx && !params) return 0;
+    float* part = params ? ws : nullptr;
+    const int rc = dtype == MADIFF_BF16 ? ln_bwd<bf16_t>((const bf16_t*)x, ldx, (const bf16_t*)dy, lddy, w, mean, rstd,
+                                                         (bf16_t*)dx, lddx, part, groups, rows, C, Cpad, stream)
+                                        : ln_bwd<float>((const float*)x, ldx, (const float*)dy, lddy, w, mean, rstd,
+                                                        (float*)dx, lddx, part, groups, rows, C, Cpad, stream);
+    if (rc) return rc;
+  }
+  if (params) {                          // rows == 0: the sums are zero (no partial is read)
+    hipLaunchKernelGGL(layer_norm_param_kernel, dim3((2 * C + 63) / 64), dim3(1024), 0, stream, ws, rows > 0 ? groups : 0, C,
+                       dw, db, accumulate);
+    MADIFF_CHECK_LAUNCH();
+  }
+  return 0;
+}

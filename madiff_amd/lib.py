@@ -84,6 +84,9 @@ _SIGS = {
     "madiff_colsum": [_i, _vp, _i, _vp, _l, _i, _vp],
     "madiff_colsum_scatter": [_i, _vp, _i, _vp, _l, _i, _vp],
     "madiff_seqsum": [_i, _vp, _i, _vp, _i, _l, _i, _i, _vp],
+    "madiff_layer_norm_fwd": [_i, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _i, _i, _f, _vp],
+    "madiff_layer_norm_groups": [_i, _l, _i],
+    "madiff_layer_norm_bwd": [_i, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _vp, _i, _vp, _l, _l, _i, _i, _vp],
     "madiff_adam_ema": [_vp, _vp, _vp, _vp, _vp, _l, _f, _f, _f, _f, _f, _f, _f, _i, _f, _vp, _vp, _i, _vp],
 }
 

@@ -190,6 +190,23 @@ class ResidualTemporalBlock(nn.Module):
         return from_cl(self.forward_cl(to_cl(x), tl, proj[:, :self.out_channels]), n, tl, self.out_channels)
 
 
+class LayerNorm(nn.Module):
+    """Layer norm over the channels, in front of a cross-agent attention (SharedConvAttentionDeconv(use_layer_norm=True));
+    forward(x) normalises the last axis of any float32 / bfloat16 tensor on the GPU."""
+
+    def __init__(self, n_channels: int, eps: float = 1e-5):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(n_channels))
+        self.bias = nn.Parameter(torch.zeros(n_channels))
+        self.n_channels, self.eps = n_channels, eps
+
+    def forward_cl(self, x):
+        return ops.layer_norm_cl(x, self.weight, self.bias, self.n_channels, self.eps)
+
+    def forward(self, x):
+        return ops.layer_norm(x, self.weight, self.bias, self.eps)
+
+
 class TemporalSelfAttention(nn.Module):
     """temporal.py:57-124: cross-agent attention with timestep-conditioned Q/K/V."""
 
@@ -214,13 +231,15 @@ class TemporalSelfAttention(nn.Module):
     def time_layers(self) -> List[nn.Linear]:
         return [self.query_time_mlp[1], self.key_time_mlp[1], self.value_time_mlp[1]]
 
-    def forward_cl(self, x, bsz, n_agents, t, time_proj):
-        """x cl [(b a) t, C]; time_proj fp32 [B*A, >= 2cq + C] = [q | k | v] time-MLP outputs."""
-        if ATTN_BLOCK_NODE:          # projection + attention core as one autograd node (ops.AttnBlock)
+    def forward_cl(self, x, bsz, n_agents, t, time_proj, norm: Optional[LayerNorm] = None):
+        """x cl [(b a) t, C]; time_proj fp32 [B*A, >= 2cq + C] = [q | k | v] time-MLP outputs.  norm: queries, keys and values
+        are projections of norm(x); the residual adds to x itself."""
+        if norm is None and ATTN_BLOCK_NODE:          # projection + attention core as one autograd node (ops.AttnBlock)
             return AttnBlock.apply(x, time_proj, self.gamma if self.residual else None, bsz, n_agents, t, self.nheads,
                                    self.cq, self.n_channels, self.residual, self.query_layer.weight, self.key_layer.weight,
                                    self.value_layer.weight, self.query_layer.bias, self.key_layer.bias, self.value_layer.bias)
-        qkv = conv_gemm(x, [self.query_layer.weight, self.key_layer.weight, self.value_layer.weight],
+        qkv = conv_gemm(x if norm is None else norm.forward_cl(x),
+                        [self.query_layer.weight, self.key_layer.weight, self.value_layer.weight],
                         [self.query_layer.bias, self.key_layer.bias, self.value_layer.bias], CONV1, t,
                         rowbias=time_proj)
         return AttnCore.apply(qkv, x, self.gamma if self.residual else None, bsz, n_agents, t, self.nheads, self.cq,
@@ -477,8 +496,6 @@ class SharedConvAttentionDeconv(nn.Module):
                  kernel_size: int = 5, residual_attn: bool = True, use_layer_norm: bool = False,
                  max_path_length: int = 100, use_temporal_attention: bool = True):
         super().__init__()
-        if use_layer_norm:
-            raise NotImplementedError("use_layer_norm is not selected by any exp_spec (SURVEY.md section 8f, row F4)")
         if not use_temporal_attention:
             # the reference builds TemporalSelfAttention layers regardless (ma_temporal.py:277-294) and then calls them
             # without the time embedding (:382,:399): its forward raises TypeError.  Nothing to be compatible with.
@@ -503,6 +520,11 @@ class SharedConvAttentionDeconv(nn.Module):
             attn.append(TemporalSelfAttention(d[1], d[1] // 16, d[1] // 4, residual=residual_attn,
                                               embed_dim=self.net.embed_dim, nheads=nhead))
         self.self_attn = nn.ModuleList(attn)
+        if use_layer_norm:                     # one norm in front of each attention (none of the exp_specs selects it)
+            self.attn_norm = nn.ModuleList([LayerNorm(a.n_channels) for a in attn])
+
+    def _norm(self, i: int) -> Optional[LayerNorm]:
+        return self.attn_norm[i] if self.use_layer_norm else None
 
     # every Linear(Mish(t_emb)) of the live graph, in execution order, evaluated by ONE GEMM per forward
     def _time_layers(self):
@@ -584,11 +606,11 @@ class SharedConvAttentionDeconv(nn.Module):
         tag = _chain_tag()
         h = net.mid_block1.forward_cl(h, t, bproj[bi], chain_out=tag); bi += 1
         h = net.mid_block2.forward_cl(h, t, bproj[bi], chain_in=tag); bi += 1
-        h = self.self_attn[0].forward_cl(h, bsz, A, t, aproj[0])
+        h = self.self_attn[0].forward_cl(h, bsz, A, t, aproj[0], self._norm(0))
         for j, (r1, r2, up) in enumerate(net.ups):
             s, ts = skips.pop()
             assert ts == t, "skip/upsample length mismatch (horizon must be divisible by 2**(levels-1))"
-            s = self.self_attn[j + 1].forward_cl(s, bsz, A, t, aproj[j + 1])
+            s = self.self_attn[j + 1].forward_cl(s, bsz, A, t, aproj[j + 1], self._norm(j + 1))
             tag = _chain_tag()
             h = r1.forward_cl(h, t, bproj[bi], x2=s, chain_out=tag); bi += 1
             h = r2.forward_cl(h, t, bproj[bi], chain_in=tag); bi += 1

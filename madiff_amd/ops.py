@@ -8,11 +8,13 @@ fails at import) - there is no PyTorch/CPU fallback on this path.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 import weakref
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import lib
 
@@ -1613,6 +1615,121 @@ class GNMish(torch.autograd.Function):
         y, gamma, beta, stats = ctx.saved_tensors
         dy, dgamma, dbeta, _, drb, dres = _gn_backward(y, gamma, beta, stats, ctx.geom, dout)
         return dy, dgamma, dbeta, drb, (dres if ctx.geom[5] == 2 else None), None, None, None, None
+
+
+# ------------------------------------------------------------------------------------------------
+# layer norm
+# ------------------------------------------------------------------------------------------------
+LAYER_NORM_MAX_COLS = 32768                # = LN_MAX_COLS of csrc/layernorm.hip
+
+
+def _device_of(t):
+    """Launches go to the current device's current stream: make the tensor's device the current one."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _rows_of(x: torch.Tensor, C: int) -> torch.Tensor:
+    """x as [rows, ...] with unit column stride and rows that do not overlap; a copy where its strides do not allow that."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if (x2.shape[1] > 1 and x2.stride(1) != 1) or (x2.shape[0] > 1 and x2.stride(0) < C):
+        x2 = x2.contiguous()
+    return x2
+
+
+def _layer_norm_forward(x, weight, bias, C, eps, stats):
+    """-> (y like x, x as rows, mean, rstd); columns behind C (pad columns of the cl format) come back as zeros."""
+    x2 = _rows_of(x, C)
+    rows, width = x2.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device).unbind(0)
+    with _device_of(x):
+        _timed("layer_norm_fwd_kernel", 0.0, lambda: lib.call(
+            "madiff_layer_norm_fwd", lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x2.data_ptr(),
+            max(x2.stride(0), width), y.data_ptr(), width, _p(weight), _p(bias), _p(mean), _p(rstd), rows, C, width, eps,
+            _stream()), nbytes=2.0 * rows * C * x.element_size())
+    return y, x2, mean, rstd
+
+
+class LayerNorm(torch.autograd.Function):
+    """apply(x, weight | None, bias | None, C, eps): layer norm over the first C columns of x's last axis."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, C: int, eps: float):
+        y, x2, mean, rstd = _layer_norm_forward(x, weight, bias, C, eps, True)
+        ctx.save_for_backward(x2, weight, bias, mean, rstd)
+        ctx.geom = (x.shape, C)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2, weight, bias, mean, rstd = ctx.saved_tensors
+        shape, C = ctx.geom
+        rows, width = x2.shape
+        dy2 = _rows_of(dy, C)
+        want = (ctx.needs_input_grad[0], weight is not None and ctx.needs_input_grad[1],
+                bias is not None and ctx.needs_input_grad[2])
+        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device) if want[0] else None
+        # parameter gradients: straight into the flat gradient where a sink is installed, else into fresh tensors
+        views = [_sink_view(p_) if w_ else None for p_, w_ in ((weight, want[1]), (bias, want[2]))]
+        live = all(v is not None and v.is_contiguous() for v, w_ in zip(views, want[1:]) if w_) and (want[1] or want[2])
+        dw, db = views if live else (torch.empty(C, dtype=torch.float32, device=x2.device) if w_ else None for w_ in want[1:])
+        dt = lib.BF16 if x2.dtype == torch.bfloat16 else lib.F32
+        with _device_of(x2):
+            n = 2 * C * lib._lib.madiff_layer_norm_groups(dt, rows, C) if want[1] or want[2] else 0
+            ws = torch.empty(n, dtype=torch.float32, device=x2.device) if n else None
+            _timed("layer_norm_bwd_kernel", 0.0, lambda: lib.call(
+                "madiff_layer_norm_bwd", dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(),
+                max(dy2.stride(0), width), _p(weight), mean.data_ptr(), rstd.data_ptr(), _p(dx), width, _p(dw), _p(db),
+                int(live), _p(ws), n, rows, C, width, _stream()), nbytes=3.0 * rows * C * x2.element_size())
+        if live:
+            for p_, v in zip((weight, bias), views):
+                if v is not None:
+                    SINK.done(p_)
+            dw = db = None
+        return dx, dw, db, None, None
+
+
+def _layer_norm_check(x, weight, bias, C, eps):
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise ValueError("layer_norm: x has to be a tensor on the GPU")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"layer_norm: x has to be float32 or bfloat16, not {x.dtype}")
+    if x.dim() < 1 or not 1 <= C <= LAYER_NORM_MAX_COLS:
+        raise ValueError(f"layer_norm: between 1 and {LAYER_NORM_MAX_COLS} columns, not shape {tuple(x.shape)}")
+    for name, p_ in (("weight", weight), ("bias", bias)):
+        if p_ is None:
+            continue
+        if p_.dtype != torch.float32:
+            raise TypeError(f"layer_norm: {name} has to be float32, not {p_.dtype}")
+        if p_.shape != (C,) or p_.device != x.device or not p_.is_contiguous():
+            raise ValueError(f"layer_norm: {name} has to be a contiguous [{C}] on {x.device}, not {tuple(p_.shape)} on {p_.device}")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"layer_norm: eps has to be finite and not negative, not {eps}")
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (float32 or bfloat16, up to 32768 columns, any
+    strides), in x's type; statistics and arithmetic are float32.  weight, bias: float32 [columns] or None.  Differentiable
+    once in all three; the same call gives the same bits."""
+    C = x.shape[-1] if torch.is_tensor(x) and x.dim() else 0
+    eps = float(eps)
+    _layer_norm_check(x, weight, bias, C, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return LayerNorm.apply(x, weight, bias, C, eps)
+    return _layer_norm_forward(x, weight, bias, C, eps, False)[0]
+
+
+def layer_norm_cl(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, C: int, eps: float = 1e-5) -> torch.Tensor:
+    """layer_norm over the C real columns of a cl matrix; its pad columns stay zero."""
+    _chk_cl(x)
+    assert x.shape[1] == pad32(C), (x.shape, C)
+    _layer_norm_check(x, weight, bias, C, eps)
+    return LayerNorm.apply(x, weight, bias, C, eps)
 
 
 def _attn_label(kind: str, A, T, H, Cq, C) -> str:
