@@ -8,7 +8,6 @@ fails at import) - there is no PyTorch/CPU fallback on this path.
 """
 from __future__ import annotations
 
-import contextlib
 import os
 import weakref
 from typing import List, Optional, Sequence, Tuple
@@ -1623,9 +1622,14 @@ class GNMish(torch.autograd.Function):
 LAYER_NORM_MAX_COLS = 32768                # = LN_MAX_COLS of csrc/layernorm.hip
 
 
-def _device_of(t):
-    """Launches go to the current device's current stream: make the tensor's device the current one."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(t: torch.Tensor, fn) -> None:
+    """fn(stream) with t's device as the current one and that device's current stream.  (The raw lookups: a tenth of the
+    time of torch.cuda.current_stream(), which is what a small call from the autograd thread would mostly be.)"""
+    dev = t.device.index
+    if torch._C._cuda_getDevice() == dev:
+        return fn(torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return fn(torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _rows_of(x: torch.Tensor, C: int) -> torch.Tensor:
@@ -1636,20 +1640,18 @@ def _rows_of(x: torch.Tensor, C: int) -> torch.Tensor:
     return x2
 
 
-def _layer_norm_forward(x, weight, bias, C, eps, stats):
-    """-> (y like x, x as rows, mean, rstd); columns behind C (pad columns of the cl format) come back as zeros."""
+def _layer_norm_forward(x, weight, bias, C, eps, want_stats):
+    """-> (y like x, x as rows, [2, rows] mean and rstd); columns behind C (pad columns of the cl format) come back as zeros."""
     x2 = _rows_of(x, C)
     rows, width = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device).unbind(0)
-    with _device_of(x):
-        _timed("layer_norm_fwd_kernel", 0.0, lambda: lib.call(
-            "madiff_layer_norm_fwd", lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x2.data_ptr(),
-            max(x2.stride(0), width), y.data_ptr(), width, _p(weight), _p(bias), _p(mean), _p(rstd), rows, C, width, eps,
-            _stream()), nbytes=2.0 * rows * C * x.element_size())
-    return y, x2, mean, rstd
+    y = torch.empty_like(x2, memory_format=torch.contiguous_format)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if want_stats else None
+    at = stats.data_ptr() if want_stats else None
+    _timed("layer_norm_fwd_kernel", 0.0, lambda: _launch(x, lambda st: lib.call(
+        "madiff_layer_norm_fwd", lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x2.data_ptr(),
+        max(x2.stride(0), width), y.data_ptr(), width, _p(weight), _p(bias), at, at + 4 * rows if want_stats else None, rows, C,
+        width, eps, st)), nbytes=2.0 * rows * C * x.element_size())
+    return y if x.dim() == 2 else y.view(x.shape), x2, stats
 
 
 class LayerNorm(torch.autograd.Function):
@@ -1657,38 +1659,45 @@ class LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, C: int, eps: float):
-        y, x2, mean, rstd = _layer_norm_forward(x, weight, bias, C, eps, True)
-        ctx.save_for_backward(x2, weight, bias, mean, rstd)
-        ctx.geom = (x.shape, C)
+        y, x2, stats = _layer_norm_forward(x, weight, bias, C, eps, True)
+        ctx.save_for_backward(x2, weight, bias, stats)
+        ctx.shape, ctx.C = x.shape, C
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2, weight, bias, mean, rstd = ctx.saved_tensors
-        shape, C = ctx.geom
+        x2, weight, bias, stats = ctx.saved_tensors
+        C = ctx.C
         rows, width = x2.shape
         dy2 = _rows_of(dy, C)
-        want = (ctx.needs_input_grad[0], weight is not None and ctx.needs_input_grad[1],
-                bias is not None and ctx.needs_input_grad[2])
-        dx = torch.empty(shape, dtype=x2.dtype, device=x2.device) if want[0] else None
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        dx = torch.empty_like(x2, memory_format=torch.contiguous_format) if want_x else None
         # parameter gradients: straight into the flat gradient where a sink is installed, else into fresh tensors
-        views = [_sink_view(p_) if w_ else None for p_, w_ in ((weight, want[1]), (bias, want[2]))]
-        live = all(v is not None and v.is_contiguous() for v, w_ in zip(views, want[1:]) if w_) and (want[1] or want[2])
-        dw, db = views if live else (torch.empty(C, dtype=torch.float32, device=x2.device) if w_ else None for w_ in want[1:])
+        dw = _sink_view(weight) if want_w else None
+        db = _sink_view(bias) if want_b else None
+        live = (want_w or want_b) and all(v is not None and v.is_contiguous()
+                                          for v, want in ((dw, want_w), (db, want_b)) if want)
         dt = lib.BF16 if x2.dtype == torch.bfloat16 else lib.F32
-        with _device_of(x2):
-            n = 2 * C * lib._lib.madiff_layer_norm_groups(dt, rows, C) if want[1] or want[2] else 0
-            ws = torch.empty(n, dtype=torch.float32, device=x2.device) if n else None
-            _timed("layer_norm_bwd_kernel", 0.0, lambda: lib.call(
-                "madiff_layer_norm_bwd", dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(),
-                max(dy2.stride(0), width), _p(weight), mean.data_ptr(), rstd.data_ptr(), _p(dx), width, _p(dw), _p(db),
-                int(live), _p(ws), n, rows, C, width, _stream()), nbytes=3.0 * rows * C * x2.element_size())
+        n, ws = 0, None
+        if want_w or want_b:
+            n = 2 * C * lib._lib.madiff_layer_norm_groups(dt, rows, C)
+            ws = torch.empty(n, dtype=torch.float32, device=x2.device)
+            if not live:
+                fresh = torch.empty(2, C, dtype=torch.float32, device=x2.device)
+                dw, db = fresh[0] if want_w else None, fresh[1] if want_b else None
+        at = stats.data_ptr()
+        _timed("layer_norm_bwd_kernel", 0.0, lambda: _launch(x2, lambda st: lib.call(
+            "madiff_layer_norm_bwd", dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(), max(dy2.stride(0), width),
+            _p(weight), at, at + 4 * rows, _p(dx), width, _p(dw), _p(db), int(live), _p(ws), n, rows, C, width, st)),
+            nbytes=3.0 * rows * C * x2.element_size())
         if live:
-            for p_, v in zip((weight, bias), views):
-                if v is not None:
+            for p_, want in ((weight, want_w), (bias, want_b)):
+                if want:
                     SINK.done(p_)
             dw = db = None
+        if dx is not None and len(ctx.shape) != 2:
+            dx = dx.view(ctx.shape)
         return dx, dw, db, None, None
 
 
