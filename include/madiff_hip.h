@@ -359,6 +359,35 @@ int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, lo
                           const float* rstd, void* dx, long lddx, float* dw, float* db, int accumulate, float* ws,
                           long ws_floats, long rows, int C, int Cpad, madiff_stream_t stream);
 
+/* Newton-Schulz orthogonalisation (no counterpart in the reference, whose optimizer is Adam): `batch` row-major matrices
+ * [rows, cols], back to back in src and in dst (dst == src is allowed), `dtype` storage.  With X = G or its transpose, short side
+ * first, over max(|G|_F, eps):  `steps` times  A = X X^T,  X <- a X + (b A + c A A) X.  Products are fp32-accurate (three fp16
+ * matrix instructions on operands kept as hi + lo), everything is summed in fp32, the norm in 64 bits.  rows, cols: the shorter up
+ * to 16384, the longer up to 2^22.  ws: madiff_ortho_ws() bytes, 256-byte aligned, used during the call only; calls that may
+ * overlap need one each. */
+int madiff_ortho_ws(int batch, int rows, int cols, long* ws_bytes);
+/* 0 when the steps of x <- x (a + b x^2 + c x^4) keep every start in [0, 1] inside what the products' operands hold (|values|
+ * < 15), steps is in 1..64 and eps > 0; -1 otherwise, and then madiff_orthogonalize / madiff_muon_step refuse the call. */
+int madiff_ortho_check(int steps, float a, float b, float c, float eps);
+int madiff_orthogonalize(int dtype, const void* src, void* dst, int batch, int rows, int cols, int steps, float a, float b,
+                         float c, float eps, void* ws, long ws_bytes, madiff_stream_t stream);
+/* Muon over a flat fp32 buffer holding n_mats matrices, matrix i row-major [rows[i], cols[i]] from element at[i] on (the matrices
+ * must not overlap; elements between them are not touched).  madiff_muon_plan lays out tables in HOST memory (plan NULL: only
+ * *need_bytes is set); the caller copies the blob to the device as it is and passes both.  scales NULL = 1.
+ * madiff_muon_plan_ws: workspace bytes of a step, and the elements the flat buffers must have.
+ * One step, for every matrix:  M <- mu M + (1 - mu) s g,  U = (1 - mu) s g + mu M (nesterov) or M,  O = orthogonalised U,
+ *   p <- decay p - lr scale O;  shadow_bf16 (or NULL) = bf16(p);  ema: 0 none, 1 lerp with ema_beta, 2 copy.
+ * momentum_rest = 1 - mu, ema_rest = 1 - ema_beta, decay = 1 - lr * weight decay: the caller forms them in 64 bits.
+ * s = grad_scale; zero_grad != 0 clears g as it is read.  state (device int[2], or NULL): the EMA mode is state[1] instead of
+ * do_ema, so that a captured step can change it. */
+int madiff_muon_plan(int n_mats, const long* at, const int* rows, const int* cols, const float* scales, void* plan,
+                     long plan_bytes, long* need_bytes);
+int madiff_muon_plan_ws(const void* plan, long* ws_bytes, long* need_elements);
+int madiff_muon_step(const void* plan, const void* plan_device, float* p, float* g, float* m, float* ema, void* shadow_bf16,
+                     long n, float lr, float momentum, float momentum_rest, int nesterov, float decay, float grad_scale,
+                     int zero_grad, int do_ema, float ema_beta, float ema_rest, const int* state, int steps, float a, float b,
+                     float c, float eps, void* ws, long ws_bytes, madiff_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

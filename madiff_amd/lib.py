@@ -87,6 +87,13 @@ _SIGS = {
     "madiff_layer_norm_fwd": [_i, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _i, _i, _f, _vp],
     "madiff_layer_norm_groups": [_i, _l, _i],
     "madiff_layer_norm_bwd": [_i, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _vp, _i, _vp, _l, _l, _i, _i, _vp],
+    "madiff_ortho_ws": [_i, _i, _i, _vp],
+    "madiff_ortho_check": [_i, _f, _f, _f, _f],
+    "madiff_orthogonalize": [_i, _vp, _vp, _i, _i, _i, _i, _f, _f, _f, _f, _vp, _l, _vp],
+    "madiff_muon_plan": [_i, _vp, _vp, _vp, _vp, _vp, _l, _vp],
+    "madiff_muon_plan_ws": [_vp, _vp, _vp],
+    "madiff_muon_step": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _f, _f, _f, _i, _f, _f, _i, _i, _f, _f, _vp, _i, _f, _f, _f, _f,
+                         _vp, _l, _vp],
     "madiff_adam_ema": [_vp, _vp, _vp, _vp, _vp, _l, _f, _f, _f, _f, _f, _f, _f, _i, _f, _vp, _vp, _i, _vp],
 }
 

@@ -8,6 +8,7 @@ fails at import) - there is no PyTorch/CPU fallback on this path.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 import weakref
 from typing import List, Optional, Sequence, Tuple
@@ -1739,6 +1740,52 @@ def layer_norm_cl(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, C: 
     assert x.shape[1] == pad32(C), (x.shape, C)
     _layer_norm_check(x, weight, bias, C, eps)
     return LayerNorm.apply(x, weight, bias, C, eps)
+
+
+# ------------------------------------------------------------------------------------------------
+# Newton-Schulz orthogonalisation
+# ------------------------------------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # the usual quintic: steep at 0, values near 1 stay within about 0.7 .. 1.2
+
+
+def _check_newton_schulz(who: str, steps, coefficients, eps):
+    a, b, c = (float(v) for v in coefficients)
+    if lib._lib.madiff_ortho_check(int(steps), a, b, c, float(eps)) != 0:
+        raise ValueError(f"{who}: steps has to be 1..64, eps positive and {steps} steps of x (a + b x^2 + c x^4) have to keep "
+                         f"[0, 1] within +-15, not steps={steps}, coefficients={tuple(coefficients)}, eps={eps}")
+    return int(steps), a, b, c, float(eps)
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float] = NEWTON_SCHULZ,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of x [..., rows, cols] (float32 or bfloat16): every matrix, over max(|x|_F, eps), goes
+    `steps` times through  X <- a X + (b A + c A A) X,  A = X X^T on its shorter side; its singular values end up near 1.
+    Products are float32-accurate whatever x's type.  Returns a new contiguous tensor of x's shape and type.  Not
+    differentiable: an update is orthogonalised outside autograd."""
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise ValueError("orthogonalize: x has to be a tensor on the GPU")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"orthogonalize: x has to be float32 or bfloat16, not {x.dtype}")
+    if x.dim() < 2:
+        raise ValueError(f"orthogonalize: x has to be [..., rows, cols], not {tuple(x.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("orthogonalize is not differentiable: call it under torch.no_grad() or on a detached tensor")
+    args = _check_newton_schulz("orthogonalize", steps, coefficients, eps)
+    rows, cols = x.shape[-2:]
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        return out
+    x = x.contiguous()
+    batch = x.numel() // (rows * cols)
+    need = ctypes.c_long()
+    if lib._lib.madiff_ortho_ws(batch, rows, cols, ctypes.byref(need)) != 0:
+        raise ValueError(f"orthogonalize: {batch} matrices of {rows} x {cols} are out of range (shorter side up to 16384, "
+                         "longer up to 4194304)")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)      # (stream-ordered, and private to a captured graph)
+    _launch(x, lambda st: lib.call(
+        "madiff_orthogonalize", lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x.data_ptr(), out.data_ptr(), batch, rows,
+        cols, *args, ws.data_ptr(), need.value, st))
+    return out
 
 
 def _attn_label(kind: str, A, T, H, Cq, C) -> str:

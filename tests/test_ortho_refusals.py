@@ -1,0 +1,90 @@
+"""What ops.orthogonalize, muon.MuonPlan and their C entry points refuse before anything is launched, and the layout of a plan
+(no GPU needed)."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def test_python_refusals():
+    from madiff_amd import ops
+    from madiff_amd.muon import MuonPlan
+    with pytest.raises(ValueError):
+        ops.orthogonalize(torch.zeros(3, 4))
+    for mats, kw in (([], {}), ([(0, 0, 4)], {}), ([(-1, 2, 2)], {}), ([(0, 3, 3), (8, 2, 2)], {}), ([(0, 2, 2)], dict(scales=[1, 2])),
+                     ([(0, 2, 2)], dict(device="cpu"))):
+        with pytest.raises(ValueError):
+            MuonPlan(mats, **kw)
+
+
+def test_c_refusals():
+    from madiff_amd import lib
+    L = lib._lib
+    ns = (3.4445, -4.7750, 2.0315)
+    assert L.madiff_ortho_check(5, *ns, 1e-7) == 0
+    for bad in ((0, *ns, 1e-7), (65, *ns, 1e-7), (5, *ns, 0.0), (5, *ns, float("nan")), (5, float("nan"), 0.0, 0.0, 1e-7),
+                (5, 16.0, 0.0, 0.0, 1e-7), (5, 4.0, -4.0, 2.5, 1e-7)):
+        assert L.madiff_ortho_check(*bad) == -1, bad
+    need = C.c_long()
+    assert L.madiff_ortho_ws(3, 100, 200, C.byref(need)) == 0 and need.value > 0 and need.value % 256 == 0
+    for bad in ((-1, 4, 4), (1, 0, 4), (1, 4, 0), (1, 16385, 16385), (1, 2, (1 << 22) + 1), (1 << 30, 128, 128)):
+        assert L.madiff_ortho_ws(*bad, C.byref(need)) == -1, bad
+    L.madiff_ortho_ws(3, 100, 200, C.byref(need))
+    p = 1 << 20
+    ok = [1, p, p, 3, 100, 200, 5, *ns, 1e-7, p, need.value, None]
+    for at, bad in ((0, 2), (1, None), (2, None), (3, -1), (4, 0), (5, 0), (6, 0), (10, 0.0), (11, None), (11, p + 16), (12, need.value - 1)):
+        args = list(ok)
+        args[at] = bad
+        assert L.madiff_orthogonalize(*args) == -1, (at, bad)
+
+
+def _plan(mats):
+    from madiff_amd import lib
+    n = len(mats)
+    at, rows, cols = (C.c_long * n)(*[m[0] for m in mats]), (C.c_int * n)(*[m[1] for m in mats]), (C.c_int * n)(*[m[2] for m in mats])
+    need = C.c_long()
+    rc = lib._lib.madiff_muon_plan(n, at, rows, cols, None, None, 0, C.byref(need))
+    if rc:
+        return rc, None
+    blob = torch.full((need.value + 64,), 7, dtype=torch.uint8)
+    assert lib._lib.madiff_muon_plan(n, at, rows, cols, None, blob.data_ptr(), need.value - 1, C.byref(need)) == -1
+    rc = lib._lib.madiff_muon_plan(n, at, rows, cols, None, blob.data_ptr(), need.value, C.byref(need))
+    assert bool((blob[need.value:] == 7).all())                         # not a byte behind what it asked for
+    return rc, blob
+
+
+def test_plan_layout_and_refusals():
+    from madiff_amd import lib
+    L = lib._lib
+    assert _plan([(0, 16385, 16385)])[0] == -1 and _plan([(-4, 2, 2)])[0] == -1 and _plan([(0, 0, 2)])[0] == -1
+    mats = [(0, 20, 300), (6000, 1, 1), (6004, 700, 129)]
+    rc, blob = _plan(mats)
+    assert rc == 0
+    ws, el = C.c_long(), C.c_long()
+    assert L.madiff_muon_plan_ws(blob.data_ptr(), C.byref(ws), C.byref(el)) == 0
+    assert el.value == 6004 + 700 * 129 and ws.value % 256 == 0
+    # every chunk, and every tile on and above the diagonal / of the long side, exactly once
+    w = blob[:112].view(torch.int64).tolist()
+    i32 = lambda lo, n: blob[lo:lo + 4 * n].view(torch.int32).tolist()                                # noqa: E731
+    n_mats, chunks, tri, full = i32(32, 4)
+    at_mats, at_chunks, at_gram, at_square, at_full = w[6:11]
+    pad = lambda v: (v + 127) // 128                                                                  # noqa: E731
+    sides = [(pad(min(r, c)), pad(max(r, c))) for _, r, c in mats]
+    ck = i32(at_chunks, 2 * chunks)
+    assert n_mats == 3 and list(zip(ck[::2], ck[1::2])) == [(i, k) for i, (_, r, c) in enumerate(mats) for k in range(-(-r * c // 16384))]
+    for at, n, want in ((at_gram, tri, [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(s) for b in range(a, s)]),
+                        (at_square, tri, [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(s) for b in range(a, s)]),
+                        (at_full, full, [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(s) for b in range(l)])):
+        t = i32(at, 4 * n)
+        got = list(zip(t[::4], t[1::4], t[2::4]))
+        assert sorted(got) == want and len(set(got)) == len(want)
+    bad = blob.clone()
+    bad[0] ^= 1
+    assert L.madiff_muon_plan_ws(bad.data_ptr(), C.byref(ws), C.byref(el)) == -1
+    p, f = 1 << 20, blob.data_ptr()
+    ok = [f, p, p, p, p, p, None, el.value, 0.1, 0.9, 0.1, 1, 1.0, 1.0, 0, 1, 0.9, 0.1, None, 5, 3.4445, -4.7750, 2.0315, 1e-7, p, ws.value, None]
+    for at, v in ((0, None), (0, bad.data_ptr()), (1, None), (2, None), (3, None), (4, None), (5, None), (7, el.value - 1), (9, 1.0), (9, -0.1),
+                  (9, float("nan")), (15, 3), (15, -1), (19, 0), (23, 0.0), (24, None), (24, p + 8), (25, ws.value - 1)):
+        args = list(ok)
+        args[at] = v
+        assert L.madiff_muon_step(*args) == -1, (at, v)
