@@ -12,10 +12,21 @@
 // are bounded (|X| <= 1.3 or so, |R| <= 5 at the usual coefficients; other coefficients are checked on the host): they
 // are stored times 2^11, which leaves values down to 2^-25 of the largest their full 22 bits.
 //
-// Storage: a matrix [R, K] (both padded with zeros to multiples of 128) holds, per row and 32 columns, 64 bytes of hi and 64
-// bytes of lo: 128-byte lines that are exactly one K-step of a tile row.  A and R are symmetric: only their tiles on and
-// above the diagonal are computed, the others are written as mirror images.
+// Storage: a matrix [R, K] (both padded with zeros to multiples of 32) is a grid of blocks of 16 rows x 16 columns, 1 KB each, a
+// row's blocks one after the other.  In a block every row has four 16-byte chunks: hi of columns 0-7, hi of 8-15, lo of 0-7, lo of
+// 8-15, in an order that depends on the row and the column block (ns_chunk), so that the straight copy of a block into LDS is free
+// of bank conflicts both for the row-wise fragment reads and for the transposing ones.  A K-step of a product is 16: whole
+// blocks, each moved by one asynchronous load instruction of a wave.  A and R are symmetric: only their tiles on and above
+// the diagonal are computed, the others are written as mirror images.
 #include "common.h"
+#include <math.h>
+#include <string.h>
+#include <algorithm>
+#include <functional>
+#include <queue>
+#include <type_traits>
+#include <utility>
+#include <vector>
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
@@ -24,11 +35,12 @@ typedef const __attribute__((address_space(1))) void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 
-#define NS_PAD 128                 // both axes of a stored matrix
+#define NS_PAD 32                  // both axes of a stored matrix
 #define NS_SCALE 2048.f            // stored value = 2^11 x
 #define NS_CHUNK 16384             // elements a workgroup of the norm pass reads
 #define NS_MAX_SHORT 16384
 #define NS_MAX_LONG (1 << 22)
+#define NS_MAX_GROUPS (1L << 23)   // workgroups of a launch: 2^31 work-items
 
 // One matrix.  Offsets into the user's buffers are in elements, into the workspace in bytes.
 struct NsMat {
@@ -40,15 +52,49 @@ struct NsMat {
   long x, sq, norm;                // X (two buffers of 4 sp lp bytes), squares (four of 4 sp sp), partials (doubles)
 };
 
-// What every kernel here gets: the matrices, the tiles, the workspace.  `list` (plan): (matrix, ti, tj, 0) per workgroup;
-// without it every matrix looks like `one` and workgroups are numbered matrix by matrix.
+// What every kernel here gets: the matrices, the tiles, the workspace.  Lists come with a plan; without
+// them every matrix looks like `one` and workgroups are numbered matrix by matrix.
 struct NsGroup {
   const NsMat* mats;
   NsMat one;
   long ws_stride, at_stride;       // bytes / elements from one matrix of the batch to the next
+  long partials;                   // where the workspace's partial sums begin, in bytes
   unsigned char* ws;
 };
 struct NsTile { int mat, ti, tj; };
+
+// Workgroups reach the 8 XCDs round-robin, each with its own L2.  The tiles of one matrix read the same rows of X (or R) at about
+// the same time, so they are given to one XCD: number `id` of `n` becomes a contiguous run per XCD.  (Plans have their lists in
+// that order already.)  The tiles of R X go through the matrix in bands of 1024 columns, all rows of a band back to back: a band
+// of X and R at one K-step is what an L2 then holds.
+__device__ __forceinline__ int ns_xcd_run(int id, int n) {
+  const int xcd = id & 7, local = id >> 3, q = n >> 3, r = n & 7;
+  return xcd * q + (xcd < r ? xcd : r) + local;
+}
+// Tile number r of a matrix.  APPLY: the whole [sp, lp]; GRAM and SQUARE: the tiles that reach the diagonal or lie above it.
+__host__ __device__ inline int ns_div_up(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ inline int ns_tiles(bool whole, int sp, int lp, int bm, int bn) {
+  const int ni = ns_div_up(sp, bm);
+  if (whole) return ni * ns_div_up(lp, bn);
+  const int nj = ns_div_up(sp, bn);
+  int n = 0;
+  for (int ti = 0; ti < ni; ti++) n += nj - ti * bm / bn;
+  return n;
+}
+__host__ __device__ inline void ns_tile_at(bool whole, int r, int sp, int lp, int bm, int bn, int& ti, int& tj) {
+  if (whole) {
+    const int ni = ns_div_up(sp, bm), nj = ns_div_up(lp, bn), wide = 1024 / bn;
+    const int band = r / (ni * wide), left = nj - band * wide, w = left < wide ? left : wide;
+    r -= band * ni * wide;
+    ti = r / w;
+    tj = band * wide + r - ti * w;
+  } else {
+    const int nj = ns_div_up(sp, bn);
+    ti = 0;
+    while (r >= nj - ti * bm / bn) { r -= nj - ti * bm / bn; ti++; }
+    tj = ti * bm / bn + r;
+  }
+}
 
 __device__ __forceinline__ NsMat ns_mat(const NsGroup& g, int mat) {
   if (g.mats) return g.mats[mat];
@@ -60,12 +106,25 @@ __device__ __forceinline__ NsMat ns_mat(const NsGroup& g, int mat) {
   return m;
 }
 
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+// byte of the 16-byte chunk holding `plane` (0 hi, 1 lo) of columns k .. k + 7 (k % 8 == 0) of row r, from the matrix's start
+__device__ __forceinline__ size_t ns_chunk(int r, int k, int plane, int kblocks) {
+  const int c = (plane * 2 + ((k >> 3) & 1)) ^ ((r >> 2) & 3) ^ ((k >> 3) & 2);
+  return ((size_t)(r >> 4) * kblocks + (k >> 4)) * 1024 + (r & 15) * 64 + c * 16;
+}
+
 __device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {      // v already scaled
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }
 
 template <int N> __device__ __forceinline__ void ns_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+template <typename F, int... I>
+__device__ __forceinline__ void ns_unroll_(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F> __device__ __forceinline__ void ns_unroll(F&& f) {
+  ns_unroll_(f, std::make_integer_sequence<int, N>{});
+}
 // 64 lanes x 16 bytes, per-lane global address -> LDS [addr + 16 lane]; addr is wave-uniform.  In asm so that the compiler's
 // waits for the fragment reads stay counted ones; ordered by the explicit vmcnt waits and barriers.
 __device__ __forceinline__ void ns_dma(const void* src, unsigned lds_addr) {
@@ -119,13 +178,12 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup grp, NsSource q, c
 template <int KIND>
 __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, const int* __restrict__ list, int per) {
   NsTile t;
-  const int tile = blockIdx.x >> 2, piece = blockIdx.x & 3;          // four pieces of a 128 x 128 tile
-  if (list) { t.mat = list[4 * tile]; t.ti = list[4 * tile + 1]; t.tj = list[4 * tile + 2]; }
+  if (list) { t.mat = list[4 * blockIdx.x]; t.ti = list[4 * blockIdx.x + 1]; t.tj = list[4 * blockIdx.x + 2]; }
   else {
-    t.mat = tile / per;
-    const int r = tile - t.mat * per, nj = grp.one.lp / NS_PAD;
-    t.ti = r / nj;
-    t.tj = r - t.ti * nj;
+    const int nj = ns_div_up(grp.one.lp, 64);
+    t.mat = blockIdx.x / per;
+    t.ti = (blockIdx.x - t.mat * per) / nj;
+    t.tj = blockIdx.x - t.mat * per - t.ti * nj;
   }
   const NsMat M = ns_mat(grp, t.mat);
   __shared__ float tilebuf[64][65];
@@ -139,7 +197,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
   __syncthreads();
   const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
   const float inv = (float)((double)NS_SCALE / (norm > (double)q.eps ? norm : (norm <= (double)q.eps ? (double)q.eps : norm)));
-  const int i0 = t.ti * 128 + (piece >> 1) * 64, j0 = t.tj * 128 + (piece & 1) * 64;   // X rows (short side), columns
+  const int i0 = t.ti * 64, j0 = t.tj * 64;   // X rows (short side), columns
   const int c = threadIdx.x & 63;
 #pragma unroll 4
   for (int k = threadIdx.x >> 6; k < 64; k += 4) {
@@ -173,9 +231,10 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
       lo[e] = l;
     }
     const int col = j0 + g8 * 8;
-    unsigned char* o = X + (size_t)(i0 + row) * M.lp * 4 + (col >> 5) * 128 + (col & 31) * 2;
-    *(f16x8*)o = hi;
-    *(f16x8*)(o + 64) = lo;
+    if (i0 + row < M.sp && col < M.lp) {
+      *(f16x8*)(X + ns_chunk(i0 + row, col, 0, M.lp >> 4)) = hi;
+      *(f16x8*)(X + ns_chunk(i0 + row, col, 1, M.lp >> 4)) = lo;
+    }
   }
 }
 
@@ -184,8 +243,8 @@ enum { NS_GRAM = 0, NS_SQUARE = 1, NS_APPLY = 2 };
 enum { NS_OUT_PLANES = 0, NS_OUT_F32 = 1, NS_OUT_BF16 = 2, NS_OUT_MUON = 3 };
 
 struct NsProduct {
-  int a, b, e1, e2, out;           // square buffers (SQUARE: A, B^T = B; addends; result) / X buffer read and written (APPLY: b, out)
-  float ca, c1, c2;                // result = ca A B + c1 E1 + c2 E2
+  int a, b, e2, out;               // square buffers (SQUARE: A, B^T = B, addend or -1, result) / X buffer read and written (APPLY: b, out)
+  float ca, c1, c2;                // result = ca A B + c1 B + c2 E2
   void* dst;                       // last APPLY: the user's buffer
   float *p, *ema;                  // Muon
   bf16_t* shadow;
@@ -194,234 +253,421 @@ struct NsProduct {
   const int* state;
 };
 
-// Tile BM x BN by WM x WN waves.  K-steps of 32: A tile [BM][hi 64 B | lo 64 B], B tile the same (products with a
-// symmetric or transposed right side) or, for R X, [32 rows of X][BN columns], read by the transposing LDS read.  D LDS stages
-// filled by asynchronous loads: step k waits (counted) for its own, passes one barrier, sends stage k + D - 1 on its way into the
-// buffer that step k - 1 has finished with, and multiplies.
-template <int KIND, int BM, int BN, int WM, int WN, int D, int OUT>
-__global__ __launch_bounds__(64 * WM * WN) void ns_product_kernel(NsGroup grp, NsProduct q, const int* __restrict__ list,
-                                                                   int per) {
-  constexpr int NW = WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
-  constexpr int A_BYTES = BM * 128, STAGE = (BM + BN) * 128;
-  constexpr int AP = BM / 8 / NW, BP = BN / 8 / NW, PIECES = AP + BP;
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole pieces a wave");
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[D * STAGE];
-  NsTile t;
-  if (list) { t.mat = list[4 * blockIdx.x]; t.ti = list[4 * blockIdx.x + 1]; t.tj = list[4 * blockIdx.x + 2]; }
-  else {
-    t.mat = blockIdx.x / per;
-    int r = blockIdx.x - t.mat * per;
-    if constexpr (KIND == NS_APPLY) {
-      const int nj = grp.one.lp / BN;
-      t.ti = r / nj;
-      t.tj = r - t.ti * nj;
+// The workgroups of one launch: tile (ti, tj) of matrix `mat`, slice `part` of `parts` of its reduction.  A tile in several parts leaves
+// fp32 partial sums at `slot` (the first part's slot: part p is at slot + p); ns_join_kernel adds them up.
+struct NsWork { int mat, ti, tj, part, parts, slot, pad0, pad1; };
+struct NsList {
+  const NsWork* work;              // null: numbered matrix by matrix, tile by tile, part by part
+  int n, tiles, parts;             // (without a list) per matrix, per tile
+};
+
+template <bool WHOLE, int BM, int BN>
+__device__ __forceinline__ NsWork ns_work(const NsGroup& g, const NsList& l, int id) {
+  if (l.work) return l.work[id];
+  NsWork w = {};
+  const int per = l.tiles * l.parts, r = id % per, tile = r % l.tiles;      // part by part: its tiles read the same columns
+  w.mat = id / per;
+  w.part = r / l.tiles;
+  w.parts = l.parts;
+  w.slot = (w.mat * l.tiles + tile) * l.parts;
+  ns_tile_at(WHOLE, tile, g.one.sp, g.one.lp, BM, BN, w.ti, w.tj);
+  return w;
+}
+
+// What becomes of a wave's 32 x 32 blocks of sums.  A lane's accumulators are groups of four columns of its row; swapping halves of
+// register pairs with the lane 32 away makes them eight, a 16-byte chunk of each plane: p = 0, 1 has columns 16 p + 8 fh .. + 7.
+// (Chunk by chunk the address units keep up; 8-byte pieces took them four times as long, a third of a tile's whole time.)
+// What the next block reads is on its way while a block is finished.  Mirror images and the user's rows are turned through a
+// piece of LDS of the wave's own.
+template <int KIND, int OUT, int BX>
+struct NsFinish {
+  struct Extra { f16x8 h1[2], l1[2], h2[2], l2[2]; f32x4 p[4], e[4]; };
+  const NsProduct& q;
+  const NsMat& M;
+  uint32_t* turn;                  // 32 x 33 words
+  const unsigned char *e1, *e2;
+  unsigned char* out;
+  int lane, rows, cols, kb, do_ema;
+  float ca;
+
+  __device__ __forceinline__ NsFinish(const NsGroup& grp, const NsProduct& q_, const NsMat& M_, uint32_t* turn_, int lane_)
+      : q(q_), M(M_), turn(turn_), lane(lane_) {
+    const size_t sq = (size_t)M.sp * M.sp * 4, xs = (size_t)M.sp * M.lp * 4;
+    rows = M.sp;
+    cols = KIND == NS_APPLY ? M.lp : M.sp;
+    kb = cols >> 4;
+    e1 = KIND == NS_APPLY ? grp.ws + M.x + q.b * xs : grp.ws + M.sq + q.b * sq;
+    e2 = KIND == NS_SQUARE && q.e2 >= 0 ? grp.ws + M.sq + q.e2 * sq : nullptr;
+    out = KIND == NS_APPLY ? grp.ws + M.x + q.out * xs : grp.ws + M.sq + q.out * sq;
+    do_ema = 0;
+    if constexpr (OUT == NS_OUT_MUON) do_ema = q.state ? q.state[1] : q.do_ema;
+    ca = q.ca * (1.f / NS_SCALE);                            // sums are in units of the scale squared
+  }
+  // The user's side of the block at (m0, n0): 32 rows of 32 columns; lane & 7 picks four columns, pass k the rows 8 k + lane / 8.
+  __device__ __forceinline__ long user(int m0, int n0, int k, int& row, int& col) const {
+    row = (M.tall ? n0 : m0) + 8 * k + (lane >> 3);
+    col = (M.tall ? m0 : n0) + 4 * (lane & 7);
+    return M.at + (long)row * M.cols + col;
+  }
+  __device__ __forceinline__ f32x4 four(const float* from, long e, int row, int col) const {
+    f32x4 d = {0.f, 0.f, 0.f, 0.f};
+    if (row < M.rows && col + 3 < M.cols) __builtin_memcpy(&d, from + e, 16);
+    else if (row < M.rows)
+#pragma unroll
+      for (int r = 0; r < 3; r++)
+        if (col + r < M.cols) d[r] = from[e + r];
+    return d;
+  }
+  template <typename T, typename V> __device__ __forceinline__ void put(T* to, const V& d, long e, int row, int col) const {
+    if (row < M.rows && col + 3 < M.cols) __builtin_memcpy(to + e, &d, sizeof d);
+    else if (row < M.rows)
+#pragma unroll
+      for (int r = 0; r < 3; r++)
+        if (col + r < M.cols) to[e + r] = d[r];
+  }
+  __device__ __forceinline__ void fetch(Extra& x, int m0, int n0) const {
+    if (m0 >= rows || n0 >= cols) return;                    // (blocks lie inside or outside as a whole)
+    if (KIND != NS_GRAM)
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const size_t at = ns_chunk(m0 + (lane & 31), n0 + 8 * (lane >> 5) + 16 * p, 0, kb);
+        x.h1[p] = *(const f16x8*)(e1 + at);
+        x.l1[p] = *(const f16x8*)(e1 + (at ^ 32));
+        if (KIND == NS_SQUARE && e2) {
+          x.h2[p] = *(const f16x8*)(e2 + at);
+          x.l2[p] = *(const f16x8*)(e2 + (at ^ 32));
+        }
+      }
+    if constexpr (OUT == NS_OUT_MUON)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        int row, col;
+        const long e = user(m0, n0, k, row, col);
+        x.p[k] = four(q.p, e, row, col);
+        if (do_ema == 1) x.e[k] = four(q.ema, e, row, col);
+      }
+  }
+  __device__ __forceinline__ void finish(const Extra& x, const f32x16& sum, int m0, int n0) const {
+    if (m0 >= rows || n0 >= cols) return;
+    const int fr = lane & 31, nl = 8 * (lane >> 5);          // this lane's row, and its columns + 16 p
+    float v[2][8];
+#pragma unroll
+    for (int p = 0; p < 2; p++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float s0 = sum[8 * p + r], s1 = sum[8 * p + 4 + r];
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(s0), __float_as_uint(s1), false, false);
+        v[p][r] = ca * __uint_as_float(w[0]);
+        v[p][4 + r] = ca * __uint_as_float(w[1]);
+      }
+    if (KIND != NS_GRAM)
+#pragma unroll
+      for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+          v[p][r] += q.c1 * ((float)x.h1[p][r] + (float)x.l1[p][r]);
+          if (KIND == NS_SQUARE && e2) v[p][r] += q.c2 * ((float)x.h2[p][r] + (float)x.l2[p][r]);
+        }
+    if constexpr (OUT == NS_OUT_PLANES) {
+      // what no tile computes: the mirror images of tiles to the right of their row of the diagonal
+      const bool mirror = KIND != NS_APPLY && m0 / BX < n0 / BX;
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        f16x8 h, l;
+        uint32_t both[8];                                    // hi | lo << 16
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+          _Float16 hh, ll;
+          ns_split(v[p][r], hh, ll);
+          h[r] = hh;
+          l[r] = ll;
+          both[r] = (uint32_t)__builtin_bit_cast(uint16_t, hh) | (uint32_t)__builtin_bit_cast(uint16_t, ll) << 16;
+        }
+        const size_t at = ns_chunk(m0 + fr, n0 + nl + 16 * p, 0, kb);
+        *(f16x8*)(out + at) = h;
+        *(f16x8*)(out + (at ^ 32)) = l;
+        if (mirror)
+#pragma unroll
+          for (int r = 0; r < 8; r++) turn[fr * 33 + nl + 16 * p + r] = both[r];
+      }
+      if (mirror) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          typedef __attribute__((ext_vector_type(8))) uint16_t u16x8;
+          u16x8 h, l;
+#pragma unroll
+          for (int r = 0; r < 8; r++) {
+            const uint32_t both = turn[(nl + 16 * p + r) * 33 + fr];
+            h[r] = (uint16_t)both;
+            l[r] = (uint16_t)(both >> 16);
+          }
+          const size_t at = ns_chunk(n0 + fr, m0 + nl + 16 * p, 0, kb);
+          *(u16x8*)(out + at) = h;
+          *(u16x8*)(out + (at ^ 32)) = l;
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
     } else {
-      const int n = grp.one.sp / BM;
-      t.ti = 0;
-      while (r >= n - t.ti) { r -= n - t.ti; t.ti++; }
-      t.tj = t.ti + r;
+      float* t = (float*)turn;
+#pragma unroll
+      for (int p = 0; p < 2; p++)
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+          const int n = nl + 16 * p + r;
+          t[M.tall ? n * 33 + fr : fr * 33 + n] = v[p][r] * (1.f / NS_SCALE);
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        int row, col;
+        const long e = user(m0, n0, k, row, col);
+        f32x4 o;
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[r] = t[(8 * k + (lane >> 3)) * 33 + 4 * (lane & 7) + r];
+        typedef __attribute__((ext_vector_type(4))) bf16_t b16x4;
+        b16x4 w16;
+        if constexpr (OUT == NS_OUT_F32) {
+          put((float*)q.dst, o, e, row, col);
+        } else if constexpr (OUT == NS_OUT_BF16) {
+#pragma unroll
+          for (int r = 0; r < 4; r++) w16[r] = (bf16_t)o[r];
+          put((bf16_t*)q.dst, w16, e, row, col);
+        } else {
+          f32x4 w, a;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            w[r] = q.decay * x.p[k][r] - q.lr * M.scale * o[r];
+            a[r] = do_ema == 1 ? q.ema_beta * x.e[k][r] + q.ema_rest * w[r] : w[r];
+            w16[r] = (bf16_t)w[r];
+          }
+          put(q.p, w, e, row, col);
+          if (do_ema) put(q.ema, a, e, row, col);
+          if (q.shadow) put(q.shadow, w16, e, row, col);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
+};
+
+// Tile BM x BN by WM x WN waves, K-steps of 16.  A stage is BM / 16 blocks of A and BN / 16 of B: for a product with a symmetric or
+// transposed right side B's rows are read like A's; for R X the blocks are those of 16 rows of X, and fragments come out of
+// the transposing LDS read.  D stages are filled by asynchronous loads.  Step k waits (counted) for stage k + 1, passes one
+// barrier, sends stage k + D - 1 on its way into the buffer whose fragments everybody has taken, reads the fragments of step
+// k + 1 and multiplies those of step k meanwhile.
+template <int KIND, int BM, int BN, int WM, int WN, int D, int OUT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp, NsProduct q, NsList list) {
+  constexpr int NW = WM * WN, TI = BM / WM / 32, TJ = BN / WN / 32, BX = BM > BN ? BM : BN;
+  constexpr int AB = BM / 16, BB = BN / 16, STAGE = (AB + BB) * 1024, PIECES = (AB + BB) / NW;
+  static_assert((AB + BB) % NW == 0 && D >= 3 && D * STAGE >= NW * 32 * 33 * 4, "whole pieces a wave");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[D * STAGE];
+  const NsWork t = ns_work<KIND == NS_APPLY, BM, BN>(grp, list, list.work ? (int)blockIdx.x : ns_xcd_run(blockIdx.x, gridDim.x));
+  if (t.mat < 0) return;           // a list's filler
   const NsMat M = ns_mat(grp, t.mat);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave - wm * WN;
   const size_t sq = (size_t)M.sp * M.sp * 4, xs = (size_t)M.sp * M.lp * 4;
-  const unsigned char *Ap, *Bp;
-  size_t lda, ldb;
-  int K;
-  if constexpr (KIND == NS_GRAM) { Ap = Bp = grp.ws + M.x + q.b * xs; lda = ldb = (size_t)M.lp * 4; K = M.lp; }
-  else if constexpr (KIND == NS_SQUARE) {
-    Ap = grp.ws + M.sq + q.a * sq;
-    Bp = grp.ws + M.sq + q.b * sq;
-    lda = ldb = (size_t)M.sp * 4;
-    K = M.sp;
-  } else {
-    Ap = grp.ws + M.sq + q.a * sq;
-    Bp = grp.ws + M.x + q.b * xs;
-    lda = (size_t)M.sp * 4;
-    ldb = (size_t)M.lp * 4;
-    K = M.sp;
-  }
+  const unsigned char* Ap = KIND == NS_GRAM ? grp.ws + M.x + q.b * xs : grp.ws + M.sq + q.a * sq;
+  const unsigned char* Bp = KIND == NS_SQUARE ? grp.ws + M.sq + q.b * sq : grp.ws + M.x + q.b * xs;
+  const int kblocks = (KIND == NS_GRAM ? M.lp : M.sp) >> 4;  // a multiple of 2
+  const int kfirst = kblocks / 2 * t.part / t.parts * 2, nsteps = kblocks / 2 * (t.part + 1) / t.parts * 2 - kfirst;
   const int i0 = t.ti * BM, j0 = t.tj * BN;
-  // source addresses of this lane's pieces for K-step 0; the LDS image is lane-linear, so the bank swizzle (chunk ^= row & 7;
-  // for the X rows a 32-byte swizzle that puts the 8 rows a half wave reads into different banks) is done on the source side
-  const unsigned char *asrc[AP], *bsrc[BP];
+  // this wave's blocks of a stage; blocks of a tile that hangs over the matrix's end repeat its last one
+  const unsigned char* src[PIECES];
+  size_t hop[PIECES];
 #pragma unroll
-  for (int j = 0; j < AP; j++) {
-    const int row = (wave * AP + j) * 8 + (lane >> 3);
-    asrc[j] = Ap + (size_t)(i0 + row) * lda + (((lane & 7) ^ (row & 7)) << 4);
-  }
-  constexpr int RB = BN * 4;                                  // bytes of a row of the X tile
-#pragma unroll
-  for (int j = 0; j < BP; j++) {
-    if constexpr (KIND == NS_APPLY) {
-      const int at = (wave * BP + j) * 1024 + lane * 16, row = at / RB, chunk = (at - row * RB) >> 4;
-      const int z = (row & 3) | ((row >> 3) & 1) << 2;
-      bsrc[j] = Bp + (size_t)row * ldb + (size_t)j0 * 4 + ((chunk ^ (z << 1)) << 4);
+  for (int j = 0; j < PIECES; j++) {
+    const int p = wave * PIECES + j;
+    if (p < AB) {
+      src[j] = Ap + (size_t)min((i0 >> 4) + p, (M.sp >> 4) - 1) * kblocks * 1024;
+      hop[j] = 1024;
+    } else if (KIND != NS_APPLY) {
+      src[j] = Bp + (size_t)min((j0 >> 4) + p - AB, (M.sp >> 4) - 1) * kblocks * 1024;
+      hop[j] = 1024;
     } else {
-      const int row = (wave * BP + j) * 8 + (lane >> 3);
-      bsrc[j] = Bp + (size_t)(j0 + row) * ldb + (((lane & 7) ^ (row & 7)) << 4);
+      src[j] = Bp + (size_t)min((j0 >> 4) + p - AB, (M.lp >> 4) - 1) * 1024;
+      hop[j] = (size_t)(M.lp >> 4) * 1024;
     }
+    src[j] += kfirst * hop[j];
   }
-  const size_t bstep = KIND == NS_APPLY ? 32 * ldb : 128;
-  const int nsteps = K >> 5;
-  auto issue = [&](int step) {
-    unsigned char* base = &smem[(step % D) * STAGE];
-#pragma unroll
-    for (int j = 0; j < AP; j++) ns_dma(asrc[j] + (size_t)step * 128, ns_lds(base + (wave * AP + j) * 1024));
-#pragma unroll
-    for (int j = 0; j < BP; j++) ns_dma(bsrc[j] + (size_t)step * bstep, ns_lds(base + A_BYTES + (wave * BP + j) * 1024));
+  auto issue = [&](int step, int buf, int j) {
+    ns_dma(src[j] + (size_t)step * hop[j] + lane * 16, ns_lds(&smem[buf * STAGE + (wave * PIECES + j) * 1024]));
   };
-  f32x4 acc[MI][NJ];
+  // fragment offsets in a stage.  Rows: lane & 31 is the row, lane >> 5 the half of the 16 columns; the other plane is 32 bytes
+  // away (xor), and odd column blocks have the planes swapped.
+  const int fr = lane & 31, fh = lane >> 5;
+  const int frag = (fr >> 4) * 1024 + (fr & 15) * 64 + ((fh ^ ((fr >> 2) & 3)) << 4);
+  const int aoff = wm * (BM / WM / 16) * 1024 + frag;
+  int boff, boff2 = 0;
+  if constexpr (KIND == NS_APPLY) {          // transposing read: 16 lanes take 4 rows x 16 columns of a block, twice
+    const int tq = (lane & 15) >> 2, tp = lane & 3, odd = (lane >> 4) & 1, r = 8 * fh + tq;
+    boff = AB * 1024 + (wn * (BN / WN / 16) + odd) * 1024 + r * 64 + (((tp >> 1) ^ (2 * fh) ^ (2 * odd)) << 4) + 8 * (tp & 1);
+    boff2 = (boff + 256) ^ 16;               // rows + 4: their chunks are one further (xor)
+  } else {
+    boff = AB * 1024 + wn * (BN / WN / 16) * 1024 + frag;
+  }
+  struct Frags { f16x8 ah[TI], al[TI], bh[TJ], bl[TJ]; };
+  constexpr int READS = TI + TJ;                              // pairs of fragment reads a step
+  auto fragment = [&](Frags& f, int buf, int odd_step, int n) {           // pair n: hi and lo of one operand block
+    const unsigned char* S = &smem[buf * STAGE];
+    const int swap = odd_step * 32;
+    if (n < TI) {
+      f.ah[n] = *(const f16x8*)(S + ((aoff ^ swap) + n * 2048));
+      f.al[n] = *(const f16x8*)(S + ((aoff ^ swap ^ 32) + n * 2048));
+    } else if constexpr (KIND == NS_APPLY) {
+      const int j = n - TI;
+      const s16x4 h0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(S + boff + j * 2048));
+      const s16x4 h1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(S + boff2 + j * 2048));
+      const s16x4 l0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(S + (boff ^ 32) + j * 2048));
+      const s16x4 l1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(S + (boff2 ^ 32) + j * 2048));
+      f.bh[j] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7));
+      f.bl[j] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int j = n - TI;
+      f.bh[j] = *(const f16x8*)(S + ((boff ^ swap) + j * 2048));
+      f.bl[j] = *(const f16x8*)(S + ((boff ^ swap ^ 32) + j * 2048));
+    }
+  };
+  f32x16 acc[TI][TJ];
 #pragma unroll
-  for (int i = 0; i < MI; i++)
+  for (int i = 0; i < TI; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  const int fr = lane & 15, fq = lane >> 4, tq = fr >> 2, tp = fr & 3;
+    for (int j = 0; j < TJ; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+  // stage k lives in buffer k % D; stages up to k + D - 2 are on their way when step k begins
 #pragma unroll
   for (int d = 0; d < D - 1; d++)
-    if (d < nsteps) issue(d);
-  for (int k = 0; k < nsteps; k++) {
-    if (k + D - 1 <= nsteps) ns_wait_vm<(D - 2) * PIECES>();
-    else ns_wait_vm<0>();
-    __builtin_amdgcn_s_barrier();
-    const unsigned char* As = &smem[(k % D) * STAGE];
-    const unsigned char* Bs = As + A_BYTES;
-    f16x8 ah[MI], al[MI], bh[NJ], bl[NJ];
+    if (d < nsteps)
 #pragma unroll
-    for (int i = 0; i < MI; i++) {
-      const int ra = wm * (BM / WM) + i * 16 + fr;
-      ah[i] = *(const f16x8*)(As + ra * 128 + ((fq ^ (ra & 7)) << 4));
-      al[i] = *(const f16x8*)(As + ra * 128 + (((fq + 4) ^ (ra & 7)) << 4));
+      for (int j = 0; j < PIECES; j++) issue(d, d, j);
+  Frags f0, f1;
+  if (nsteps >= D - 1) ns_wait_vm<(D - 2) * PIECES>();
+  else ns_wait_vm<0>();
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int n = 0; n < READS; n++) fragment(f0, 0, 0, n);
+  int buf = 0;                                               // of step k
+  // One step.  Operands swapped: a lane then holds groups of four consecutive columns of one row.  The three products of an
+  // accumulator are a tile's worth of instructions apart (back to back, each would wait for the one before it), and the
+  // next step's fragment reads and the loads of stage k + D - 1 are dealt out between them: issued in one go, they kept every
+  // wave from its matrix instructions for a third to a half of a step more.
+  auto step = [&](auto steady, int k, Frags& c, Frags& n, int odd_next) {
+    constexpr bool STEADY = decltype(steady)::value;
+    const int next = buf + 1 == D ? 0 : buf + 1, last = buf == 0 ? D - 1 : buf - 1;
+    const bool more = STEADY || k + 1 < nsteps, send = STEADY || k + D - 1 < nsteps;
+    if (more) {
+      // stages k + 1 .. k + D - 2 may be outstanding: D - 3 of them may stay so
+      if (STEADY || k + D - 1 <= nsteps) ns_wait_vm<(D - 3) * PIECES>();
+      else ns_wait_vm<0>();
+      __builtin_amdgcn_s_barrier();    // every wave has the fragments of step k - 1: stage k + D - 1 takes that step's buffer
     }
+    if constexpr (!STEADY) {
+      if (send)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      if constexpr (KIND == NS_APPLY) {
-        const int r0 = 8 * fq + tq, z = (r0 & 3) | ((r0 >> 3) & 1) << 2;    // (the same for row r0 + 4)
-        const int cb = wn * (BN / WN / 16) + j, c = (cb >> 1) * 8 + (cb & 1) * 2 + (tp >> 1), o = 8 * (tp & 1);
-        const unsigned char* h0 = Bs + r0 * RB + ((c ^ (z << 1)) << 4) + o;
-        const unsigned char* l0 = Bs + r0 * RB + (((c + 4) ^ (z << 1)) << 4) + o;
-        const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)h0);
-        const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(h0 + 4 * RB));
-        const s16x4 b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)l0);
-        const s16x4 b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(l0 + 4 * RB));
-        bh[j] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-        bl[j] = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
-      } else {
-        const int rb = wn * (BN / WN) + j * 16 + fr;
-        bh[j] = *(const f16x8*)(Bs + rb * 128 + ((fq ^ (rb & 7)) << 4));
-        bl[j] = *(const f16x8*)(Bs + rb * 128 + (((fq + 4) ^ (rb & 7)) << 4));
+        for (int j = 0; j < PIECES; j++) issue(k + D - 1, last, j);
+      if (more)
+#pragma unroll
+        for (int e = 0; e < READS; e++) fragment(n, next, odd_next, e);
+    }
+    constexpr int TOTAL = 3 * TI * TJ;
+#pragma unroll
+    for (int m = 0; m < TOTAL; m++) {
+      const int part = m / (TI * TJ), i = m % (TI * TJ) / TJ, j = m % TJ;
+      if constexpr (STEADY) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < READS; e++)
+          if (e * TOTAL / READS == m) fragment(n, next, odd_next, e);
+#pragma unroll
+        for (int e = 0; e < PIECES; e++)
+          if ((2 * e + 1) * TOTAL / (2 * PIECES) == m) issue(k + D - 1, last, e);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(part == 0 ? c.bl[j] : c.bh[j], part == 1 ? c.al[i] : c.ah[i], acc[i][j], 0, 0, 0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    if (k + D - 1 < nsteps) issue(k + D - 1);
-    __builtin_amdgcn_sched_barrier(0);
-    // operands swapped: a lane then holds four consecutive columns of one row
-#pragma unroll
-    for (int i = 0; i < MI; i++)
-#pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bl[j], ah[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh[j], al[i], acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bh[j], ah[i], acc[i][j], 0, 0, 0);
-      }
-  }
-
-  // ---- epilogue, in units of the stored scale
-  const float ca = q.ca * (1.f / NS_SCALE);
-  const unsigned char *e1 = nullptr, *e2 = nullptr;
-  size_t lde;
-  unsigned char* out;
-  if constexpr (KIND == NS_APPLY) {
-    e1 = grp.ws + M.x + q.b * xs;
-    lde = (size_t)M.lp * 4;
-    out = grp.ws + M.x + q.out * xs;
-  } else {
-    if (KIND == NS_SQUARE) {
-      e1 = grp.ws + M.sq + q.e1 * sq;
-      if (q.e2 >= 0) e2 = grp.ws + M.sq + q.e2 * sq;
-    }
-    lde = (size_t)M.sp * 4;
-    out = grp.ws + M.sq + q.out * sq;
-  }
-  const bool mirror = KIND != NS_APPLY && t.ti != t.tj;
-  int do_ema = 0;
-  if constexpr (OUT == NS_OUT_MUON) do_ema = q.state ? q.state[1] : q.do_ema;
-  auto addend = [&](const unsigned char* e, int m, int n) {
-    const unsigned char* a = e + (size_t)m * lde + (n >> 5) * 128 + (n & 31) * 2;
-    const f16x4 h = *(const f16x4*)a, l = *(const f16x4*)(a + 64);
-    f32x4 v;
-#pragma unroll
-    for (int r = 0; r < 4; r++) v[r] = (float)h[r] + (float)l[r];
-    return v;
+    buf = next;
   };
+  int k = 0;
+  for (; k + D < nsteps; k += 2) {
+    step(std::true_type{}, k, f0, f1, 1);
+    step(std::true_type{}, k + 1, f1, f0, 0);
+  }
+  for (; k < nsteps; k += 2) {
+    step(std::false_type{}, k, f0, f1, 1);
+    step(std::false_type{}, k + 1, f1, f0, 0);
+  }
+  const int m0 = i0 + wm * (BM / WM), n0 = j0 + wn * (BN / WN);
+  if (t.parts > 1) {                                         // this part's sums, as the lanes hold them
+    float* to = (float*)(grp.ws + grp.partials) + (size_t)(t.slot + t.part) * (BM * BN) + (size_t)wave * (TI * TJ * 1024) + lane * 4;
+    ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {
+      constexpr int b = decltype(at)::value;
 #pragma unroll
-  for (int i = 0; i < MI; i++)
+      for (int g = 0; g < 4; g++) {
+        f32x4 v;
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const int m = i0 + wm * (BM / WM) + i * 16 + fr, n = j0 + wn * (BN / WN) + j * 16 + 4 * fq;
-      f32x4 v;
-#pragma unroll
-      for (int r = 0; r < 4; r++) v[r] = ca * acc[i][j][r];
-      if (KIND != NS_GRAM) {
-        const f32x4 w = addend(e1, m, n);
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] += q.c1 * w[r];
+        for (int r = 0; r < 4; r++) v[r] = acc[b / TJ][b % TJ][4 * g + r];
+        *(f32x4*)(to + b * 1024 + g * 256) = v;
       }
-      if (KIND == NS_SQUARE && e2) {
-        const f32x4 w = addend(e2, m, n);
+    });
+    return;
+  }
+  __syncthreads();                                           // the stages are free from here on
+  const NsFinish<KIND, OUT, BX> fin(grp, q, M, (uint32_t*)smem + wave * (32 * 33), lane);
+  typename NsFinish<KIND, OUT, BX>::Extra x0, x1;
+  fin.fetch(x0, m0, n0);
+  ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {      // (acc lives in registers: its indices are constants)
+    constexpr int t0 = decltype(at)::value, t1 = t0 + 1;
+    auto &now = t0 & 1 ? x1 : x0, &then = t0 & 1 ? x0 : x1;
+    if constexpr (t1 < TI * TJ) fin.fetch(then, m0 + t1 / TJ * 32, n0 + t1 % TJ * 32);
+    fin.finish(now, acc[t0 / TJ][t0 % TJ], m0 + t0 / TJ * 32, n0 + t0 % TJ * 32);
+  });
+}
+
+// Tiles whose reduction was cut: the partial sums in part order, then the same ending.  One wave for one wave's row of blocks.
+template <int KIND, int BM, int BN, int WM, int WN, int OUT>
+__global__ __launch_bounds__(64) void ns_join_kernel(NsGroup grp, NsProduct q, NsList list) {
+  constexpr int NW = WM * WN, TI = BM / WM / 32, TJ = BN / WN / 32, BX = BM > BN ? BM : BN;
+  __shared__ uint32_t turn[32 * 33];
+  const int id = blockIdx.x / (NW * TI), sub = blockIdx.x % (NW * TI), wave = sub / TI, i = sub % TI, lane = threadIdx.x;
+  NsWork t;
+  if (list.work) {
+    t = list.work[id];
+  } else {                                                   // tiles matrix by matrix: their first part
+    t = ns_work<KIND == NS_APPLY, BM, BN>(grp, list, id / list.tiles * list.tiles * list.parts + id % list.tiles);
+  }
+  const NsMat M = ns_mat(grp, t.mat);
+  const float* from = (const float*)(grp.ws + grp.partials) + (size_t)t.slot * (BM * BN) + (size_t)wave * (TI * TJ * 1024) +
+                      i * (TJ * 1024) + lane * 4;
+  const int m0 = t.ti * BM + wave / WN * (BM / WM) + i * 32, n0 = t.tj * BN + wave % WN * (BN / WN);
+  const NsFinish<KIND, OUT, BX> fin(grp, q, M, turn, lane);
 #pragma unroll
-        for (int r = 0; r < 4; r++) v[r] += q.c2 * w[r];
+  for (int j = 0; j < TJ; j++) {
+    typename NsFinish<KIND, OUT, BX>::Extra x;
+    fin.fetch(x, m0, n0 + j * 32);
+    f32x16 sum;
+#pragma unroll
+    for (int r = 0; r < 16; r++) sum[r] = 0.f;
+    for (int p = 0; p < t.parts; p++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f32x4 v = *(const f32x4*)(from + (size_t)p * (BM * BN) + j * 1024 + g * 256);
+#pragma unroll
+        for (int r = 0; r < 4; r++) sum[4 * g + r] += v[r];
       }
-      if constexpr (OUT == NS_OUT_PLANES) {
-        f16x4 h, l;
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          _Float16 hh, ll;
-          ns_split(v[r], hh, ll);
-          h[r] = hh;
-          l[r] = ll;
-        }
-        unsigned char* o = out + (size_t)m * lde + (n >> 5) * 128 + (n & 31) * 2;
-        *(f16x4*)o = h;
-        *(f16x4*)(o + 64) = l;
-        if (mirror)
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            unsigned char* om = out + (size_t)(n + r) * lde + (m >> 5) * 128 + (m & 31) * 2;
-            *(_Float16*)om = h[r];
-            *(_Float16*)(om + 64) = l[r];
-          }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int row = M.tall ? n + r : m, col = M.tall ? m : n + r;
-          if (row >= M.rows || col >= M.cols) continue;
-          const long e = M.at + (long)row * M.cols + col;
-          const float o = v[r] * (1.f / NS_SCALE);
-          if constexpr (OUT == NS_OUT_F32) ((float*)q.dst)[e] = o;
-          else if constexpr (OUT == NS_OUT_BF16) ((bf16_t*)q.dst)[e] = (bf16_t)o;
-          else {
-            const float w = q.decay * q.p[e] - q.lr * M.scale * o;
-            q.p[e] = w;
-            if (q.shadow) q.shadow[e] = (bf16_t)w;
-            if (do_ema == 1) q.ema[e] = q.ema_beta * q.ema[e] + q.ema_rest * w;
-            else if (do_ema == 2) q.ema[e] = w;
-          }
-        }
-      }
-    }
+    fin.finish(x, sum, m0, n0 + j * 32);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct NsPlan {                    // start of a plan; lists and matrices follow
-  long magic, bytes, ws_bytes, need;      // need: elements the flat buffers must have
-  int mats, chunks, tri, full;
-  long at_mats, at_chunks, at_gram, at_square, at_full;
+struct NsPlan {                    // start of a plan; matrices and lists follow
+  long magic, bytes, ws_bytes, need, partials;       // need: elements the flat buffers must have
+  int mats, chunks, areas, shape[3], works[3], joins[3];
+  long at_mats, at_chunks, at_areas, at_works[3], at_joins[3];
 };
-static const long NS_MAGIC = 0x6d7501;
+static const long NS_MAGIC = 0x6d7502;
 
-static inline int ns_up(int v) { return (v + NS_PAD - 1) / NS_PAD * NS_PAD; }
 static bool ns_describe(NsMat& m, long at, int rows, int cols, float scale, long& ws) {
   if (rows < 1 || cols < 1 || at < 0) return false;
   m.at = at;
@@ -431,8 +677,8 @@ static bool ns_describe(NsMat& m, long at, int rows, int cols, float scale, long
   m.s = m.tall ? cols : rows;
   m.l = m.tall ? rows : cols;
   if (m.s > NS_MAX_SHORT || m.l > NS_MAX_LONG) return false;
-  m.sp = ns_up(m.s);
-  m.lp = ns_up(m.l);
+  m.sp = ns_div_up(m.s, NS_PAD) * NS_PAD;
+  m.lp = ns_div_up(m.l, NS_PAD) * NS_PAD;
   const long parts = ((long)rows * cols + NS_CHUNK - 1) / NS_CHUNK;
   m.parts = (int)parts;
   m.scale = scale;
@@ -446,18 +692,70 @@ static bool ns_describe(NsMat& m, long at, int rows, int cols, float scale, long
   return true;
 }
 
-struct NsRun {                     // one call: the group, its lists, its launch sizes
+// ---- which tile, and how many parts.  Two tile shapes; what one workgroup takes, in microseconds, as measured on an MI355X: a K-step
+// with two workgroups on every CU and with one, the rest of a tile (first loads, ending), the same for a part.  64 x 64 gives
+// the most workgroups (5 of 256 x 2048: A A 6.2 us where 128 x 128 takes 11.8), 128 x 128 loads half as much for the same work
+// (28 of 1024 x 1024: R X 189 us where 64 x 64 takes 275).  256 x 256 with one workgroup a CU reaches four fifths of the matrix rate in
+// its loop but loses it again to its ending and to unfilled rounds (200 us there), 128 x 256 likewise: neither is kept.  Parts pay
+// where there are few tiles (1024 x 5120 alone: A = X X^T 82 us whole, 21 + 8 us in six parts).
+struct NsShape { int bm, bn; double full, alone, rest, part; };
+static const NsShape ns_shapes[2] = {{64, 64, 0.25, 0.127, 4.0, 3.0}, {128, 128, 0.70, 0.39, 8.0, 5.0}};
+static inline int ns_ksteps(int kind, int sp, int lp) { return (kind == NS_GRAM ? lp : sp) / 16; }
+static inline int ns_tiles_of(int kind, int shape, int sp, int lp) {
+  return ns_tiles(kind == NS_APPLY, sp, lp, ns_shapes[shape].bm, ns_shapes[shape].bn);
+}
+static inline int ns_parts(int ksteps, int len) {             // parts of about `len` steps, two at least each
+  const int most = ksteps / 2, p = (ksteps + len / 2) / len;
+  return p < 1 ? 1 : (p > most ? most : (p > 64 ? 64 : p));
+}
+static inline double ns_tile_time(const NsShape& s, int ksteps, int parts, bool alone) {
+  return (double)ksteps / parts * (alone ? s.alone : s.full) + (parts > 1 ? s.part : s.rest);
+}
+static inline double ns_join_time(const NsShape& s, double parts) {   // a launch, and the partial sums written and read
+  return parts > 0 ? 4.5 + parts * s.bm * s.bn * 4 / 4.5e6 : 0.0;
+}
+static const int NS_SLOTS = 512;                              // two workgroups a CU
+static const int ns_lens[] = {1 << 30, 512, 320, 256, 192, 160, 128, 112, 96, 80, 64, 56, 48, 40, 32, 24, 16, 12, 8};
+
+// `batch` equal matrices
+static void ns_choose(int kind, int batch, int sp, int lp, int& shape, int& parts) {
+  const int ks = ns_ksteps(kind, sp, lp);
+  double best = -1.0;
+  for (int s = 0; s < 2; s++)
+    for (int len : ns_lens) {
+      const int p = ns_parts(ks, len);
+      const double tiles = (double)batch * ns_tiles_of(kind, s, sp, lp), n = tiles * p;
+      if (n > (double)NS_MAX_GROUPS) continue;             // (one part a tile of 64 x 64 always fits)
+      const double rounds = n <= NS_SLOTS ? 1.0 : n / NS_SLOTS + 0.25;
+      const double t = rounds * ns_tile_time(ns_shapes[s], ks, p, n <= 256.0) + ns_join_time(ns_shapes[s], p > 1 ? n : 0.0);
+      if (best < 0.0 || t < best) { best = t; shape = s; parts = p; }
+    }
+}
+
+struct NsRun {                     // one call
   NsGroup grp;
-  const int *chunks, *gram, *square, *full;
-  int n_chunks, n_tri, n_full;     // workgroups over all matrices
-  int per_chunks, per_tri, per_full;
+  const int *chunks, *areas;       // norm and split passes: (matrix, chunk), (matrix, ti, tj, 0); null: numbered
+  int n_chunks, per_chunks, n_areas, per_areas;
+  int shape[3], joins[3];          // joins: tiles in several parts
+  NsList work[3], join[3];
 };
 
+template <int KIND, int OUT, int BM, int BN, int D>
+static void ns_go(const NsRun& r, const NsProduct& q, hipStream_t st) {
+  hipLaunchKernelGGL((ns_product_kernel<KIND, BM, BN, 2, 2, D, OUT>), dim3(r.work[KIND].n), dim3(256), 0, st, r.grp, q, r.work[KIND]);
+  if (r.joins[KIND] > 0)
+    hipLaunchKernelGGL((ns_join_kernel<KIND, BM, BN, 2, 2, OUT>), dim3(r.joins[KIND] * (BM / 16)), dim3(64), 0, st, r.grp, q,
+                       r.join[KIND]);
+}
 template <int KIND, int OUT>
 static void ns_launch(const NsRun& r, const NsProduct& q, hipStream_t st) {
-  const int* list = KIND == NS_APPLY ? r.full : KIND == NS_GRAM ? r.gram : r.square;
-  hipLaunchKernelGGL((ns_product_kernel<KIND, 128, 128, 2, 2, 2, OUT>), dim3(KIND == NS_APPLY ? r.n_full : r.n_tri), dim3(256), 0,
-                     st, r.grp, q, list, KIND == NS_APPLY ? r.per_full : r.per_tri);
+  if (r.shape[KIND] == 1) ns_go<KIND, OUT, 128, 128, 4>(r, q, st);
+  else ns_go<KIND, OUT, 64, 64, 8>(r, q, st);
+}
+template <int KIND>
+static void ns_launch_source(const NsRun& r, const NsSource& q, hipStream_t st) {
+  hipLaunchKernelGGL((ns_norm_kernel<KIND>), dim3(r.n_chunks), dim3(256), 0, st, r.grp, q, r.chunks, r.per_chunks);
+  hipLaunchKernelGGL((ns_split_kernel<KIND>), dim3(r.n_areas), dim3(256), 0, st, r.grp, q, r.areas, r.per_areas);
 }
 
 // out: NS_OUT_F32 / BF16 / MUON for the last product; `last` holds its destination
@@ -471,12 +769,12 @@ static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int 
     q.ca = 1.f;
     q.e2 = -1;
     ns_launch<NS_GRAM, NS_OUT_PLANES>(r, q, st);
-    q.a = q.b = q.e1 = G;
+    q.a = q.b = G;                                           // R = b G + c G G
     q.out = R;
     q.ca = c;
     q.c1 = b;
     ns_launch<NS_SQUARE, NS_OUT_PLANES>(r, q, st);
-    q = k == steps - 1 ? last : q;
+    q = k == steps - 1 ? last : NsProduct{};
     q.a = R;
     q.b = x;
     q.out = x ^ 1;
@@ -496,6 +794,7 @@ static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int 
 // The polynomial's orbit from every start in [0, 1]: the largest |x|, |A| and |R| on it have to stay in the stored range.
 static bool ns_bounded(int steps, float a, float b, float c) {
   const double top = 65504.0 / NS_SCALE / 2;
+  if (!(fabsf(a) < top)) return false;
   for (int i = 0; i <= 4096; i++) {
     double x = (double)i / 4096;
     for (int k = 0; k < steps; k++) {
@@ -511,48 +810,55 @@ extern "C" int madiff_ortho_check(int steps, float a, float b, float c, float ep
   return steps >= 1 && steps <= 64 && eps > 0.f && eps < 1e30f && ns_bounded(steps, a, b, c) ? 0 : -1;
 }
 
-extern "C" int madiff_ortho_ws(int batch, int rows, int cols, long* ws_bytes) {
-  NsMat m;
+// Everything about a call on `batch` equal matrices but its pointers
+static int ns_uniform(int batch, int rows, int cols, NsRun& r, long& ws_bytes) {
+  NsMat& m = r.grp.one;
   long ws = 0;
-  if (batch < 0 || !ws_bytes || !ns_describe(m, 0, rows, cols, 1.f, ws)) return -1;
-  const long tiles = (long)(m.sp / NS_PAD) * (m.lp / NS_PAD);
-  if (batch > 0 && (tiles * 4 > 0x7fffffffL / batch || m.parts > 0x7fffffffL / batch)) return -1;
-  *ws_bytes = ws * batch;
+  if (batch < 0 || !ns_describe(m, 0, rows, cols, 1.f, ws)) return -1;
+  const long areas = (long)ns_div_up(m.sp, 64) * ns_div_up(m.lp, 64);
+  if (batch > 0 && (areas > NS_MAX_GROUPS / batch || m.parts > NS_MAX_GROUPS / batch)) return -1;
+  r.grp.ws_stride = ws;
+  r.grp.at_stride = (long)rows * cols;
+  r.grp.partials = ws * batch;
+  r.per_chunks = m.parts;
+  r.n_chunks = batch * m.parts;
+  r.per_areas = (int)areas;
+  r.n_areas = batch * (int)areas;
+  long slots = 0;
+  for (int k = 0; k < 3; k++) {
+    int parts = 1;
+    ns_choose(k, batch, m.sp, m.lp, r.shape[k], parts);
+    const int tiles = ns_tiles_of(k, r.shape[k], m.sp, m.lp);
+    r.work[k] = {nullptr, batch * tiles * parts, tiles, parts};
+    r.join[k] = r.work[k];
+    r.joins[k] = parts > 1 ? batch * tiles : 0;
+    const long bytes = parts > 1 ? (long)r.work[k].n * ns_shapes[r.shape[k]].bm * ns_shapes[r.shape[k]].bn * 4 : 0;
+    slots = bytes > slots ? bytes : slots;
+  }
+  ws_bytes = ws * batch + slots;
   return 0;
+}
+
+extern "C" int madiff_ortho_ws(int batch, int rows, int cols, long* ws_bytes) {
+  NsRun r = {};
+  return ws_bytes ? ns_uniform(batch, rows, cols, r, *ws_bytes) : -1;
 }
 
 extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int batch, int rows, int cols, int steps, float a,
                                     float b, float c, float eps, void* ws, long ws_bytes, hipStream_t stream) {
+  NsRun r = {};
   long need = 0;
-  if ((dtype != MADIFF_F32 && dtype != MADIFF_BF16) || madiff_ortho_ws(batch, rows, cols, &need) ||
+  if ((dtype != MADIFF_F32 && dtype != MADIFF_BF16) || ns_uniform(batch, rows, cols, r, need) ||
       madiff_ortho_check(steps, a, b, c, eps))
     return -1;
   if (batch == 0) return 0;
   if (!src || !dst || !ws || ws_bytes < need || ((size_t)ws & 255)) return -1;
-  NsRun r = {};
-  long stride = 0;
-  ns_describe(r.grp.one, 0, rows, cols, 1.f, stride);
-  const NsMat& m = r.grp.one;
-  r.grp.ws_stride = stride;
-  r.grp.at_stride = (long)rows * cols;
   r.grp.ws = (unsigned char*)ws;
-  const int ni = m.sp / NS_PAD;
-  r.per_chunks = m.parts;
-  r.per_tri = ni * (ni + 1) / 2;
-  r.per_full = ni * (m.lp / NS_PAD);
-  r.n_chunks = batch * r.per_chunks;
-  r.n_tri = batch * r.per_tri;
-  r.n_full = batch * r.per_full;
   NsSource q = {};
   q.src = src;
   q.eps = eps;
-  if (dtype == MADIFF_BF16) {
-    hipLaunchKernelGGL((ns_norm_kernel<1>), dim3(r.n_chunks), dim3(256), 0, stream, r.grp, q, (const int*)nullptr, r.per_chunks);
-    hipLaunchKernelGGL((ns_split_kernel<1>), dim3(4 * r.n_full), dim3(256), 0, stream, r.grp, q, (const int*)nullptr, r.per_full);
-  } else {
-    hipLaunchKernelGGL((ns_norm_kernel<0>), dim3(r.n_chunks), dim3(256), 0, stream, r.grp, q, (const int*)nullptr, r.per_chunks);
-    hipLaunchKernelGGL((ns_split_kernel<0>), dim3(4 * r.n_full), dim3(256), 0, stream, r.grp, q, (const int*)nullptr, r.per_full);
-  }
+  if (dtype == MADIFF_BF16) ns_launch_source<1>(r, q, stream);
+  else ns_launch_source<0>(r, q, stream);
   MADIFF_CHECK_LAUNCH();
   NsProduct last = {};
   last.dst = dst;
@@ -560,70 +866,175 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
 }
 
 // ---- Muon plans: a host blob that is copied to the device as it is
-extern "C" int madiff_muon_plan(int n, const long* at, const int* rows, const int* cols, const float* scales, void* plan,
-                                long plan_bytes, long* need_bytes) {
-  if (n < 1 || !at || !rows || !cols || !need_bytes) return -1;
-  long ws = 0, chunks = 0, tri = 0, full = 0, need = 0;
-  for (int i = 0; i < n; i++) {
-    NsMat m;
-    if (!ns_describe(m, at[i], rows[i], cols[i], 1.f, ws)) return -1;
-    const long ni = m.sp / NS_PAD;
-    chunks += m.parts;
-    tri += ni * (ni + 1) / 2;
-    full += ni * (m.lp / NS_PAD);
-    const long end = m.at + (long)m.rows * m.cols;
-    need = end > need ? end : need;
-    if (chunks > 0x10000000L || tri > 0x10000000L || full > 0x10000000L) return -1;
+namespace {
+// What the chip needs for a product over all matrices with a tile shape and a part length: list scheduling, longest first
+double ns_plan_time(const std::vector<NsMat>& mats, int kind, int shape, int len) {
+  const NsShape& s = ns_shapes[shape];
+  std::vector<std::pair<double, long>> runs;                 // duration, how many
+  double n = 0.0, joined = 0.0;
+  for (const NsMat& m : mats) n += (double)ns_tiles_of(kind, shape, m.sp, m.lp) * ns_parts(ns_ksteps(kind, m.sp, m.lp), len);
+  double total = 0.0;
+  for (const NsMat& m : mats) {
+    const int ks = ns_ksteps(kind, m.sp, m.lp), p = ns_parts(ks, len);
+    const long c = (long)ns_tiles_of(kind, shape, m.sp, m.lp) * p;
+    const double d = ns_tile_time(s, ks, p, n <= 256.0);
+    runs.push_back({d, c});
+    total += d * c;
+    if (p > 1) joined += c;
   }
+  double end = total / NS_SLOTS;
+  if (n < 20000.0) {
+    std::sort(runs.begin(), runs.end(), [](auto& x, auto& y) { return x.first > y.first; });
+    std::priority_queue<double, std::vector<double>, std::greater<double>> free;
+    for (int i = 0; i < NS_SLOTS; i++) free.push(0.0);
+    end = 0.0;
+    for (const auto& r : runs)
+      for (long i = 0; i < r.second; i++) {
+        const double t = free.top() + r.first;
+        free.pop();
+        free.push(t);
+        end = t > end ? t : end;
+      }
+  }
+  return end + ns_join_time(s, joined);
+}
+
+// The order of one list: runs of neighbouring tiles of a matrix go to the XCD with the least work so far, the costly runs first;
+// the XCDs' queues, long reductions first, are then dealt out in turn (workgroup i starts on XCD i % 8), mat = -1 filling the gaps.
+int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out, std::vector<NsWork>& joins, long& partial_bytes) {
+  int shape = 0, len = 1 << 30;
+  double best = -1.0;
+  for (int s = 0; s < 2; s++)
+    for (int l : ns_lens) {
+      const double t = ns_plan_time(mats, kind, s, l);
+      if (best < 0.0 || t < best) { best = t; shape = s; len = l; }
+    }
+  const NsShape& sh = ns_shapes[shape];
+  struct Run { int mat, lo, hi; double cost; };              // works [lo, hi) of a matrix: part by part, tile by tile
+  std::vector<Run> runs;
+  std::vector<std::vector<NsWork>> works(mats.size());
+  double total = 0.0;
+  int slots = 0;
+  auto cost = [&](const NsWork& w) {
+    return ns_tile_time(sh, ns_ksteps(kind, mats[w.mat].sp, mats[w.mat].lp), w.parts, false);
+  };
+  for (int i = 0; i < (int)mats.size(); i++) {
+    const NsMat& m = mats[i];
+    const int tiles = ns_tiles_of(kind, shape, m.sp, m.lp), parts = ns_parts(ns_ksteps(kind, m.sp, m.lp), len);
+    for (int p = 0; p < parts; p++)
+      for (int t = 0; t < tiles; t++) {
+        NsWork w = {i, 0, 0, p, parts, parts > 1 ? slots + t * parts : 0, 0, 0};
+        ns_tile_at(kind == NS_APPLY, t, m.sp, m.lp, sh.bm, sh.bn, w.ti, w.tj);
+        works[i].push_back(w);
+        if (p == 0 && parts > 1) joins.push_back(w);
+        total += cost(w);
+      }
+    if (parts > 1) slots += tiles * parts;
+  }
+  partial_bytes = (long)slots * sh.bm * sh.bn * 4;
+  for (int i = 0; i < (int)mats.size(); i++) {
+    const double c = cost(works[i][0]);
+    const int n = (int)works[i].size();
+    int most = (int)(total / 32 / c);
+    most = most < 1 ? 1 : (most > 64 ? 64 : most);
+    for (int lo = 0; lo < n; lo += most) {
+      const int hi = lo + most < n ? lo + most : n;
+      runs.push_back({i, lo, hi, c * (hi - lo)});
+    }
+  }
+  std::stable_sort(runs.begin(), runs.end(), [](const Run& x, const Run& y) { return x.cost > y.cost; });
+  std::vector<NsWork> queue[8];
+  double load[8] = {};
+  for (const Run& r : runs) {
+    int x = 0;
+    for (int y = 1; y < 8; y++)
+      if (load[y] < load[x]) x = y;
+    load[x] += r.cost;
+    queue[x].insert(queue[x].end(), works[r.mat].begin() + r.lo, works[r.mat].begin() + r.hi);
+  }
+  size_t longest = 0;
+  for (auto& x : queue) {
+    std::stable_sort(x.begin(), x.end(), [&](const NsWork& p, const NsWork& q) { return cost(p) > cost(q); });
+    longest = x.size() > longest ? x.size() : longest;
+  }
+  const NsWork none = {-1, 0, 0, 0, 1, 0, 0, 0};
+  for (size_t at = 0; at < longest; at++)
+    for (auto& x : queue) out.push_back(at < x.size() ? x[at] : none);
+  while (!out.empty() && out.back().mat < 0) out.pop_back();
+  return shape;
+}
+
+int ns_plan(int n, const long* at, const int* rows, const int* cols, const float* scales, void* plan, long plan_bytes,
+            long* need_bytes) {
+  std::vector<NsMat> mats(n);
+  long ws = 0, chunks = 0, need = 0, areas = 0, partials = 0;
+  for (int i = 0; i < n; i++) {
+    if (!ns_describe(mats[i], at[i], rows[i], cols[i], scales ? scales[i] : 1.f, ws)) return -1;
+    chunks += mats[i].parts;
+    areas += (long)ns_div_up(mats[i].sp, 64) * ns_div_up(mats[i].lp, 64);
+    const long end = mats[i].at + (long)rows[i] * cols[i];
+    need = end > need ? end : need;
+    if (chunks > NS_MAX_GROUPS || areas > NS_MAX_GROUPS) return -1;
+  }
+  std::vector<NsWork> work[3], join[3];
   NsPlan h = {};
+  for (int k = 0; k < 3; k++) {
+    long bytes = 0;
+    h.shape[k] = ns_order(mats, k, work[k], join[k], bytes);
+    h.works[k] = (int)work[k].size();
+    h.joins[k] = (int)join[k].size();
+    partials = bytes > partials ? bytes : partials;
+  }
   h.magic = NS_MAGIC;
-  h.ws_bytes = ws;
+  h.partials = ws;
+  h.ws_bytes = ws + partials;
   h.need = need;
   h.mats = n;
   h.chunks = (int)chunks;
-  h.tri = (int)tri;
-  h.full = (int)full;
-  h.at_mats = 256;
-  h.at_chunks = h.at_mats + (long)n * sizeof(NsMat);
-  h.at_gram = (h.at_chunks + chunks * 8 + 15) / 16 * 16;
-  h.at_square = h.at_gram + tri * 16;
-  h.at_full = h.at_square + tri * 16;
-  h.bytes = h.at_full + full * 16;
+  h.areas = (int)areas;
+  long end = 256;
+  auto take = [&](long bytes) {
+    const long from = end;
+    end += (bytes + 31) / 32 * 32;
+    return from;
+  };
+  h.at_mats = take((long)n * sizeof(NsMat));
+  h.at_chunks = take(chunks * 8);
+  h.at_areas = take(areas * 16);
+  for (int k = 0; k < 3; k++) {
+    h.at_works[k] = take((long)h.works[k] * sizeof(NsWork));
+    h.at_joins[k] = take((long)h.joins[k] * sizeof(NsWork));
+  }
+  h.bytes = end;
   *need_bytes = h.bytes;
   if (!plan) return 0;
   if (plan_bytes < h.bytes) return -1;
   unsigned char* out = (unsigned char*)plan;
-  *(NsPlan*)out = h;
-  NsMat* mats = (NsMat*)(out + h.at_mats);
-  int* ck = (int*)(out + h.at_chunks);
-  ws = 0;
+  memset(out, 0, h.bytes);
+  memcpy(out, &h, sizeof h);
+  memcpy(out + h.at_mats, mats.data(), (size_t)n * sizeof(NsMat));
+  int *ck = (int*)(out + h.at_chunks), *ar = (int*)(out + h.at_areas);
   for (int i = 0; i < n; i++) {
-    ns_describe(mats[i], at[i], rows[i], cols[i], scales ? scales[i] : 1.f, ws);
     for (int p = 0; p < mats[i].parts; p++) { *ck++ = i; *ck++ = p; }
+    for (int ti = 0; ti < ns_div_up(mats[i].sp, 64); ti++)
+      for (int tj = 0; tj < ns_div_up(mats[i].lp, 64); tj++) { *ar++ = i; *ar++ = ti; *ar++ = tj; *ar++ = 0; }
   }
-  int* lists[3] = {(int*)(out + h.at_gram), (int*)(out + h.at_square), (int*)(out + h.at_full)};
-  // the tiles with the longest reduction first: they are the last to finish when they start last
-  for (int w = 0; w < 3; w++) {
-    int* o = lists[w];
-    long bound = -1;                                          // lengths in falling order, matrices in the given order
-    for (;;) {
-      long next = -1;
-      for (int i = 0; i < n; i++) {
-        const long k = w == 0 ? mats[i].lp : mats[i].sp;
-        if ((bound < 0 || k < bound) && k > next) next = k;
-      }
-      if (next < 0) break;
-      for (int i = 0; i < n; i++) {
-        const NsMat& m = mats[i];
-        if ((w == 0 ? m.lp : m.sp) != next) continue;
-        const int ni = m.sp / NS_PAD, nj = m.lp / NS_PAD;
-        for (int ti = 0; ti < ni; ti++)
-          for (int tj = w == 2 ? 0 : ti; tj < (w == 2 ? nj : ni); tj++) { *o++ = i; *o++ = ti; *o++ = tj; *o++ = 0; }
-      }
-      bound = next;
-    }
+  for (int k = 0; k < 3; k++) {
+    memcpy(out + h.at_works[k], work[k].data(), work[k].size() * sizeof(NsWork));
+    if (!join[k].empty()) memcpy(out + h.at_joins[k], join[k].data(), join[k].size() * sizeof(NsWork));
   }
   return 0;
+}
+}  // namespace
+
+extern "C" int madiff_muon_plan(int n, const long* at, const int* rows, const int* cols, const float* scales, void* plan,
+                                long plan_bytes, long* need_bytes) {
+  if (n < 1 || !at || !rows || !cols || !need_bytes) return -1;
+  try {
+    return ns_plan(n, at, rows, cols, scales, plan, plan_bytes, need_bytes);
+  } catch (...) {                  // out of host memory: nothing leaves a C entry by an exception
+    return -1;
+  }
 }
 
 extern "C" int madiff_muon_plan_ws(const void* plan, long* ws_bytes, long* need_elements) {
@@ -647,13 +1058,18 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   NsRun r = {};
   r.grp.mats = (const NsMat*)(dev + h->at_mats);
   r.grp.ws = (unsigned char*)ws;
+  r.grp.partials = h->partials;
   r.chunks = (const int*)(dev + h->at_chunks);
-  r.gram = (const int*)(dev + h->at_gram);
-  r.square = (const int*)(dev + h->at_square);
-  r.full = (const int*)(dev + h->at_full);
+  r.areas = (const int*)(dev + h->at_areas);
   r.n_chunks = h->chunks;
-  r.n_tri = h->tri;
-  r.n_full = h->full;
+  r.n_areas = h->areas;
+  r.per_chunks = r.per_areas = 1;
+  for (int k = 0; k < 3; k++) {
+    r.shape[k] = h->shape[k];
+    r.joins[k] = h->joins[k];
+    r.work[k] = {(const NsWork*)(dev + h->at_works[k]), h->works[k], 1, 1};
+    r.join[k] = {(const NsWork*)(dev + h->at_joins[k]), h->joins[k], 1, 1};
+  }
   NsSource q = {};
   q.g = g;
   q.m = m;
@@ -663,8 +1079,7 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   q.nesterov = nesterov;
   q.zero_grad = zero_grad;
   q.eps = eps;
-  hipLaunchKernelGGL((ns_norm_kernel<2>), dim3(r.n_chunks), dim3(256), 0, stream, r.grp, q, r.chunks, 1);
-  hipLaunchKernelGGL((ns_split_kernel<2>), dim3(4 * r.n_full), dim3(256), 0, stream, r.grp, q, r.full, 1);
+  ns_launch_source<2>(r, q, stream);
   MADIFF_CHECK_LAUNCH();
   NsProduct last = {};
   last.p = p;

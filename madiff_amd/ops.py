@@ -1745,6 +1745,7 @@ def layer_norm_cl(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, C: 
 # ------------------------------------------------------------------------------------------------
 # Newton-Schulz orthogonalisation
 # ------------------------------------------------------------------------------------------------
+ORTHO_WS_BYTES, ORTHO_MAX_BATCH = 16 << 30, 65536      # a larger batch goes in several calls
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # the usual quintic: steep at 0, values near 1 stay within about 0.7 .. 1.2
 
 
@@ -1778,13 +1779,21 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     x = x.contiguous()
     batch = x.numel() // (rows * cols)
     need = ctypes.c_long()
-    if lib._lib.madiff_ortho_ws(batch, rows, cols, ctypes.byref(need)) != 0:
-        raise ValueError(f"orthogonalize: {batch} matrices of {rows} x {cols} are out of range (shorter side up to 16384, "
-                         "longer up to 4194304)")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)      # (stream-ordered, and private to a captured graph)
-    _launch(x, lambda st: lib.call(
-        "madiff_orthogonalize", lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x.data_ptr(), out.data_ptr(), batch, rows,
-        cols, *args, ws.data_ptr(), need.value, st))
+    if lib._lib.madiff_ortho_ws(1, rows, cols, ctypes.byref(need)) != 0:
+        raise ValueError(f"orthogonalize: matrices of {rows} x {cols} are out of range (shorter side up to 16384, longer up to "
+                         "4194304)")
+    dt, es = (lib.BF16 if x.dtype == torch.bfloat16 else lib.F32), x.element_size()
+    most = max(1, min(batch, ORTHO_WS_BYTES // need.value, ORTHO_MAX_BATCH))          # matrices a call
+    while lib._lib.madiff_ortho_ws(most, rows, cols, ctypes.byref(need)) != 0:
+        most = (most + 1) // 2
+    for lo in range(0, batch, most):
+        n = min(most, batch - lo)
+        if n != most:
+            lib.call("madiff_ortho_ws", n, rows, cols, ctypes.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)  # (stream-ordered, and private to a captured graph)
+        at = lo * rows * cols * es
+        _launch(x, lambda st: lib.call("madiff_orthogonalize", dt, x.data_ptr() + at, out.data_ptr() + at, n, rows, cols, *args,
+                                       ws.data_ptr(), need.value, st))
     return out
 
 

@@ -64,20 +64,36 @@ def test_plan_layout_and_refusals():
     assert L.madiff_muon_plan_ws(blob.data_ptr(), C.byref(ws), C.byref(el)) == 0
     assert el.value == 6004 + 700 * 129 and ws.value % 256 == 0
     # every chunk, and every tile on and above the diagonal / of the long side, exactly once
-    w = blob[:112].view(torch.int64).tolist()
+    w = blob[:256].view(torch.int64).tolist()
     i32 = lambda lo, n: blob[lo:lo + 4 * n].view(torch.int32).tolist()                                # noqa: E731
-    n_mats, chunks, tri, full = i32(32, 4)
-    at_mats, at_chunks, at_gram, at_square, at_full = w[6:11]
-    pad = lambda v: (v + 127) // 128                                                                  # noqa: E731
-    sides = [(pad(min(r, c)), pad(max(r, c))) for _, r, c in mats]
+    n_mats, chunks, areas, *rest = i32(40, 12)
+    shapes, works, joins = rest[:3], rest[3:6], rest[6:9]
+    at_mats, at_chunks, at_areas = w[11:14]
+    at_works, at_joins = w[14:17], w[17:20]
+    up = lambda v, d: -(-v // d)                                                                      # noqa: E731
+    sides = [(32 * up(min(r, c), 32), 32 * up(max(r, c), 32)) for _, r, c in mats]
     ck = i32(at_chunks, 2 * chunks)
-    assert n_mats == 3 and list(zip(ck[::2], ck[1::2])) == [(i, k) for i, (_, r, c) in enumerate(mats) for k in range(-(-r * c // 16384))]
-    for at, n, want in ((at_gram, tri, [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(s) for b in range(a, s)]),
-                        (at_square, tri, [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(s) for b in range(a, s)]),
-                        (at_full, full, [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(s) for b in range(l)])):
-        t = i32(at, 4 * n)
-        got = list(zip(t[::4], t[1::4], t[2::4]))
-        assert sorted(got) == want and len(set(got)) == len(want)
+    assert n_mats == 3 and list(zip(ck[::2], ck[1::2])) == [(i, k) for i, (_, r, c) in enumerate(mats) for k in range(up(r * c, 16384))]
+    ar = i32(at_areas, 4 * areas)
+    assert list(zip(ar[::4], ar[1::4], ar[2::4])) == [(i, a, b) for i, (s, l) in enumerate(sides) for a in range(up(s, 64))
+                                                      for b in range(up(l, 64))]
+    for kind in range(3):
+        b = (64, 128)[shapes[kind]]
+        want = {(i, x, y) for i, (s, l) in enumerate(sides) for x in range(up(s, b)) for y in (range(up(l, b)) if kind == 2 else range(x, up(s, b)))}
+        t = i32(at_works[kind], 8 * works[kind])
+        got = [t[8 * k:8 * k + 6] for k in range(works[kind]) if t[8 * k] != -1]          # (-1: filler)
+        parts, slots = {}, set()
+        for m, x, y, part, n, slot in got:
+            assert (part, n) not in parts.setdefault((m, x, y), []) and 0 <= part < n
+            parts[(m, x, y)].append((part, n))
+            if n > 1:
+                assert slot + part not in slots                          # no two parts share a slot
+                slots.add(slot + part)
+        assert set(parts) == want and all(len(v) == v[0][1] for v in parts.values())
+        t = i32(at_joins[kind], 8 * joins[kind])
+        joined = [tuple(t[8 * k:8 * k + 3]) for k in range(joins[kind])]
+        assert sorted(joined) == sorted(k for k, v in parts.items() if len(v) > 1)
+        assert (max(slots, default=-1) + 1) * b * b * 4 + w[4] <= ws.value
     bad = blob.clone()
     bad[0] ^= 1
     assert L.madiff_muon_plan_ws(bad.data_ptr(), C.byref(ws), C.byref(el)) == -1
