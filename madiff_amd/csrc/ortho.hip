@@ -40,7 +40,7 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 #define NS_CHUNK 16384             // elements a workgroup of the norm pass reads
 #define NS_MAX_SHORT 16384
 #define NS_MAX_LONG (1 << 22)
-#define NS_MAX_GROUPS (1L << 23)   // workgroups of a launch: 2^31 work-items
+#define NS_MAX_GROUPS (1L << 21)   // workgroups of a launch: 2^31 work-items of 1024-lane ones
 
 // One matrix.  Offsets into the user's buffers are in elements, into the workspace in bytes.
 struct NsMat {
@@ -146,31 +146,70 @@ struct NsSource {
 
 // Partial sums of squares in 64 bits (no gradient is too small or too large), one per NS_CHUNK elements.  Muon: the momentum
 // update M <- mu M + (1 - mu) g on the way, and the squares are those of U = (1 - mu) g + mu M (Nesterov) or M.
+// Four (eight) consecutive elements a lane and pass, all of a chunk's passes in flight together.
 template <int KIND>                // 0 fp32, 1 bf16, 2 Muon
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsGroup grp, NsSource q, const int* __restrict__ chunks, int per) {
+__global__ __launch_bounds__(1024) void ns_norm_kernel(NsGroup grp, NsSource q, const int* __restrict__ chunks, int per) {
   int mat, chunk;
   if (chunks) { mat = chunks[2 * blockIdx.x]; chunk = chunks[2 * blockIdx.x + 1]; }
   else { mat = blockIdx.x / per; chunk = blockIdx.x - mat * per; }
   const NsMat M = ns_mat(grp, mat);
   const long n = (long)M.rows * M.cols, lo = (long)chunk * NS_CHUNK, hi = min(n, lo + NS_CHUNK);
+  constexpr int V = KIND == 1 ? 8 : 4, PASSES = NS_CHUNK / 1024 / V;
   double sum = 0.0;
-  for (long e = lo + threadIdx.x; e < hi; e += 256) {
-    float v;
-    if constexpr (KIND == 2) {
-      const float g = q.g[M.at + e] * q.grad_scale, m = q.mu * q.m[M.at + e] + q.rest * g;
-      q.m[M.at + e] = m;
-      v = q.nesterov ? q.rest * g + q.mu * m : m;
-    } else {
-      v = KIND == 1 ? to_f32(((const bf16_t*)q.src)[M.at + e]) : ((const float*)q.src)[M.at + e];
+  auto take = [&](float v) { sum += (double)v * (double)v; };
+  auto step = [&](float g, float m) {                        // -> the new momentum
+    const float now = q.mu * m + q.rest * (g * q.grad_scale);
+    take(q.nesterov ? q.rest * (g * q.grad_scale) + q.mu * now : now);
+    return now;
+  };
+  if (lo + NS_CHUNK <= n) {
+    typedef __attribute__((ext_vector_type(4))) float f4;
+    f4 a[PASSES], b[PASSES];
+    const long at = M.at + lo + threadIdx.x * V;
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {                       // (element-aligned addresses: the hardware takes them)
+      if constexpr (KIND == 2) {
+        __builtin_memcpy(&a[p], q.g + at + p * 1024 * V, 16);
+        __builtin_memcpy(&b[p], q.m + at + p * 1024 * V, 16);
+      } else if constexpr (KIND == 1) {
+        __builtin_memcpy(&a[p], (const bf16_t*)q.src + at + p * 1024 * V, 16);
+      } else {
+        __builtin_memcpy(&a[p], (const float*)q.src + at + p * 1024 * V, 16);
+      }
     }
-    sum += (double)v * (double)v;
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+      if constexpr (KIND == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) b[p][e] = step(a[p][e], b[p][e]);
+        __builtin_memcpy(q.m + at + p * 1024 * V, &b[p], 16);
+      } else if constexpr (KIND == 1) {
+        bf16_t h[8];
+        __builtin_memcpy(h, &a[p], 16);
+#pragma unroll
+        for (int e = 0; e < 8; e++) take(to_f32(h[e]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) take(a[p][e]);
+      }
+    }
+  } else {
+    for (long e = lo + threadIdx.x; e < hi; e += 1024) {
+      if constexpr (KIND == 2) q.m[M.at + e] = step(q.g[M.at + e], q.m[M.at + e]);
+      else take(KIND == 1 ? to_f32(((const bf16_t*)q.src)[M.at + e]) : ((const float*)q.src)[M.at + e]);
+    }
   }
-  __shared__ double lds[4];
+  __shared__ double lds[16];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) ((double*)(grp.ws + M.norm))[chunk] = lds[0] + lds[1] + lds[2] + lds[3];
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) sum += lds[w];
+    ((double*)(grp.ws + M.norm))[chunk] = sum;
+  }
 }
 
 // X0 = U / max(|U|, eps) in split form, padding included; a 64 x 64 piece of X a workgroup, through LDS so that the source is
@@ -188,6 +227,23 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
   const NsMat M = ns_mat(grp, t.mat);
   __shared__ float tilebuf[64][65];
   __shared__ double part[4];
+  const int i0 = t.ti * 64, j0 = t.tj * 64;                  // X rows (short side), columns
+  const int c = threadIdx.x & 63, k0 = threadIdx.x >> 6;
+  float v[16];
+#pragma unroll
+  for (int u = 0; u < 16; u++) {                             // the piece is on its way while the norm is put together
+    const int r = (M.tall ? j0 : i0) + k0 + 4 * u, col = (M.tall ? i0 : j0) + c;         // in the user's orientation
+    v[u] = 0.f;
+    if (r < M.rows && col < M.cols) {
+      const long e = M.at + (long)r * M.cols + col;
+      if constexpr (KIND == 2) {
+        const float m = q.m[e];
+        v[u] = q.nesterov ? q.rest * (q.g[e] * q.grad_scale) + q.mu * m : m;
+      } else {
+        v[u] = KIND == 1 ? to_f32(((const bf16_t*)q.src)[e]) : ((const float*)q.src)[e];
+      }
+    }
+  }
   double sum = 0.0;
   const double* parts = (const double*)(grp.ws + M.norm);
   for (int i = threadIdx.x; i < M.parts; i += 256) sum += parts[i];
@@ -197,25 +253,15 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
   __syncthreads();
   const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
   const float inv = (float)((double)NS_SCALE / (norm > (double)q.eps ? norm : (norm <= (double)q.eps ? (double)q.eps : norm)));
-  const int i0 = t.ti * 64, j0 = t.tj * 64;   // X rows (short side), columns
-  const int c = threadIdx.x & 63;
-#pragma unroll 4
-  for (int k = threadIdx.x >> 6; k < 64; k += 4) {
-    const int r = M.tall ? j0 + k : i0 + k, col = M.tall ? i0 + c : j0 + c;            // in the user's orientation
-    float v = 0.f;
-    if (r < M.rows && col < M.cols) {
-      const long e = M.at + (long)r * M.cols + col;
-      if constexpr (KIND == 2) {
-        const float m = q.m[e];
-        v = q.nesterov ? q.rest * (q.g[e] * q.grad_scale) + q.mu * m : m;
-        if (q.zero_grad) q.g[e] = 0.f;
-      } else {
-        v = KIND == 1 ? to_f32(((const bf16_t*)q.src)[e]) : ((const float*)q.src)[e];
-      }
-      v *= inv;
+#pragma unroll
+  for (int u = 0; u < 16; u++) {
+    const int k = k0 + 4 * u;
+    if (M.tall) tilebuf[c][k] = v[u] * inv;
+    else tilebuf[k][c] = v[u] * inv;
+    if constexpr (KIND == 2) {
+      const int r = (M.tall ? j0 : i0) + k, col = (M.tall ? i0 : j0) + c;
+      if (q.zero_grad && r < M.rows && col < M.cols) q.g[M.at + (long)r * M.cols + col] = 0.f;
     }
-    if (M.tall) tilebuf[c][k] = v;
-    else tilebuf[k][c] = v;
   }
   __syncthreads();
   unsigned char* X = grp.ws + M.x;
@@ -663,7 +709,7 @@ __global__ __launch_bounds__(64) void ns_join_kernel(NsGroup grp, NsProduct q, N
 // ------------------------------------------------------------------------------------------------ host
 struct NsPlan {                    // start of a plan; matrices and lists follow
   long magic, bytes, ws_bytes, need, partials;       // need: elements the flat buffers must have
-  int mats, chunks, areas, shape[3], works[3], joins[3];
+  int mats, chunks, areas, shape[3], works[3], joins[3], pairs, pad_;
   long at_mats, at_chunks, at_areas, at_works[3], at_joins[3];
 };
 static const long NS_MAGIC = 0x6d7502;
@@ -718,7 +764,7 @@ static const int NS_SLOTS = 512;                              // two workgroups 
 static const int ns_lens[] = {1 << 30, 512, 320, 256, 192, 160, 128, 112, 96, 80, 64, 56, 48, 40, 32, 24, 16, 12, 8};
 
 // `batch` equal matrices
-static void ns_choose(int kind, int batch, int sp, int lp, int& shape, int& parts) {
+static double ns_choose(int kind, int batch, int sp, int lp, int& shape, int& parts) {
   const int ks = ns_ksteps(kind, sp, lp);
   double best = -1.0;
   for (int s = 0; s < 2; s++)
@@ -730,13 +776,18 @@ static void ns_choose(int kind, int batch, int sp, int lp, int& shape, int& part
       const double t = rounds * ns_tile_time(ns_shapes[s], ks, p, n <= 256.0) + ns_join_time(ns_shapes[s], p > 1 ? n : 0.0);
       if (best < 0.0 || t < best) { best = t; shape = s; parts = p; }
     }
+  return best;
 }
+
+// one A and one pass over X saved against four square products more
+static inline bool ns_pairs(const double (&time)[3]) { return time[NS_GRAM] + time[NS_APPLY] > 4.0 * time[NS_SQUARE]; }
 
 struct NsRun {                     // one call
   NsGroup grp;
   const int *chunks, *areas;       // norm and split passes: (matrix, chunk), (matrix, ti, tj, 0); null: numbered
   int n_chunks, per_chunks, n_areas, per_areas;
   int shape[3], joins[3];          // joins: tiles in several parts
+  bool pairs;                      // two steps in one go are the faster
   NsList work[3], join[3];
 };
 
@@ -754,34 +805,53 @@ static void ns_launch(const NsRun& r, const NsProduct& q, hipStream_t st) {
 }
 template <int KIND>
 static void ns_launch_source(const NsRun& r, const NsSource& q, hipStream_t st) {
-  hipLaunchKernelGGL((ns_norm_kernel<KIND>), dim3(r.n_chunks), dim3(256), 0, st, r.grp, q, r.chunks, r.per_chunks);
+  hipLaunchKernelGGL((ns_norm_kernel<KIND>), dim3(r.n_chunks), dim3(1024), 0, st, r.grp, q, r.chunks, r.per_chunks);
   hipLaunchKernelGGL((ns_split_kernel<KIND>), dim3(r.n_areas), dim3(256), 0, st, r.grp, q, r.areas, r.per_areas);
 }
 
-// out: NS_OUT_F32 / BF16 / MUON for the last product; `last` holds its destination
-static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int out, const NsProduct& last, hipStream_t st) {
-  enum { G = 0, R = 1 };
+// out: NS_OUT_F32 / BF16 / MUON for the last product; `last` holds its destination.
+// pairs: two steps share one A = X X^T and one product with X.  With R = b A + c A A and everything a polynomial in A,
+//   A' = (a + R)^2 A = a T + R T,  T = a A + R A        R' = b A' + c A' A'        X'' = a^2 X + P X,  P = R' R + a R + a R'
+// six square products for two and two passes over X for four.  A' carries the rounding of A rather than that of a new X X^T: the
+// result is 1.3 to 1.8 times as far from the 64-bit one as step by step, which is nothing next to a rounding to bf16 or an
+// update of fp32 weights, and is not done for an fp32 result.
+static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int out, const NsProduct& last, bool pairs,
+                      hipStream_t st) {
+  enum { G = 0, R = 1, T = 2, R2 = 3 };
+  auto square = [&](int x, int y, float ca, float c1, int e2, float c2, int to) {        // to = ca x y + c1 y + c2 e2
+    NsProduct q = {};
+    q.a = x;
+    q.b = y;
+    q.ca = ca;
+    q.c1 = c1;
+    q.e2 = e2;
+    q.c2 = c2;
+    q.out = to;
+    ns_launch<NS_SQUARE, NS_OUT_PLANES>(r, q, st);
+  };
   int x = 0;
-  for (int k = 0; k < steps; k++) {
+  for (int k = 0; k < steps;) {
+    const bool two = pairs && k + 2 <= steps;
     NsProduct q = {};
     q.b = x;
     q.out = G;
     q.ca = 1.f;
-    q.e2 = -1;
     ns_launch<NS_GRAM, NS_OUT_PLANES>(r, q, st);
-    q.a = q.b = G;                                           // R = b G + c G G
-    q.out = R;
-    q.ca = c;
-    q.c1 = b;
-    ns_launch<NS_SQUARE, NS_OUT_PLANES>(r, q, st);
-    q = k == steps - 1 ? last : NsProduct{};
-    q.a = R;
+    square(G, G, c, b, -1, 0.f, R);
+    if (two) {
+      square(R, G, 1.f, a, -1, 0.f, T);
+      square(R, T, 1.f, a, -1, 0.f, G);
+      square(G, G, c, b, -1, 0.f, R2);
+      square(R2, R, 1.f, a, R2, a, T);
+    }
+    k += two ? 2 : 1;
+    q = k >= steps ? last : NsProduct{};
+    q.a = two ? T : R;
     q.b = x;
     q.out = x ^ 1;
     q.ca = 1.f;
-    q.c1 = a;
-    q.e2 = -1;
-    if (k < steps - 1) ns_launch<NS_APPLY, NS_OUT_PLANES>(r, q, st);
+    q.c1 = two ? a * a : a;
+    if (k < steps) ns_launch<NS_APPLY, NS_OUT_PLANES>(r, q, st);
     else if (out == NS_OUT_F32) ns_launch<NS_APPLY, NS_OUT_F32>(r, q, st);
     else if (out == NS_OUT_BF16) ns_launch<NS_APPLY, NS_OUT_BF16>(r, q, st);
     else ns_launch<NS_APPLY, NS_OUT_MUON>(r, q, st);
@@ -791,23 +861,26 @@ static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int 
   return 0;
 }
 
-// The polynomial's orbit from every start in [0, 1]: the largest |x|, |A| and |R| on it have to stay in the stored range.
-static bool ns_bounded(int steps, float a, float b, float c) {
+// The polynomial's orbit from every start in [0, 1]: the largest |x|, |A| and |R| on it, and what pairs of steps store besides,
+// have to stay in the stored range.
+static bool ns_bounded(int steps, float a, float b, float c, bool pairs) {
   const double top = 65504.0 / NS_SCALE / 2;
-  if (!(fabsf(a) < top)) return false;
+  auto in = [&](double v) { return v < top && v > -top; };
   for (int i = 0; i <= 4096; i++) {
-    double x = (double)i / 4096;
+    double x = (double)i / 4096, before = 0.0;
     for (int k = 0; k < steps; k++) {
       const double g = x * x, q = b * g + c * g * g;
       x = x * (a + q);
-      if (!(x < top && x > -top && g < top && q < top && q > -top)) return false;
+      if (!(in(x) && in(g) && in(q))) return false;
+      if (pairs && !(in((a + q) * g) && (k % 2 == 0 || in((a + q) * (a + before) - (double)a * a)))) return false;
+      before = q;
     }
   }
   return true;
 }
 
 extern "C" int madiff_ortho_check(int steps, float a, float b, float c, float eps) {
-  return steps >= 1 && steps <= 64 && eps > 0.f && eps < 1e30f && ns_bounded(steps, a, b, c) ? 0 : -1;
+  return steps >= 1 && steps <= 64 && eps > 0.f && eps < 1e30f && ns_bounded(steps, a, b, c, false) ? 0 : -1;
 }
 
 // Everything about a call on `batch` equal matrices but its pointers
@@ -825,9 +898,10 @@ static int ns_uniform(int batch, int rows, int cols, NsRun& r, long& ws_bytes) {
   r.per_areas = (int)areas;
   r.n_areas = batch * (int)areas;
   long slots = 0;
+  double time[3];
   for (int k = 0; k < 3; k++) {
     int parts = 1;
-    ns_choose(k, batch, m.sp, m.lp, r.shape[k], parts);
+    time[k] = ns_choose(k, batch, m.sp, m.lp, r.shape[k], parts);
     const int tiles = ns_tiles_of(k, r.shape[k], m.sp, m.lp);
     r.work[k] = {nullptr, batch * tiles * parts, tiles, parts};
     r.join[k] = r.work[k];
@@ -835,6 +909,7 @@ static int ns_uniform(int batch, int rows, int cols, NsRun& r, long& ws_bytes) {
     const long bytes = parts > 1 ? (long)r.work[k].n * ns_shapes[r.shape[k]].bm * ns_shapes[r.shape[k]].bn * 4 : 0;
     slots = bytes > slots ? bytes : slots;
   }
+  r.pairs = ns_pairs(time);
   ws_bytes = ws * batch + slots;
   return 0;
 }
@@ -862,7 +937,8 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
   MADIFF_CHECK_LAUNCH();
   NsProduct last = {};
   last.dst = dst;
-  return ns_iterate(r, steps, a, b, c, dtype == MADIFF_BF16 ? NS_OUT_BF16 : NS_OUT_F32, last, stream);
+  const bool pairs = dtype == MADIFF_BF16 && r.pairs && ns_bounded(steps, a, b, c, true);
+  return ns_iterate(r, steps, a, b, c, dtype == MADIFF_BF16 ? NS_OUT_BF16 : NS_OUT_F32, last, pairs, stream);
 }
 
 // ---- Muon plans: a host blob that is copied to the device as it is
@@ -883,7 +959,7 @@ double ns_plan_time(const std::vector<NsMat>& mats, int kind, int shape, int len
     if (p > 1) joined += c;
   }
   double end = total / NS_SLOTS;
-  if (n < 20000.0) {
+  if (n < 3000.0) {
     std::sort(runs.begin(), runs.end(), [](auto& x, auto& y) { return x.first > y.first; });
     std::priority_queue<double, std::vector<double>, std::greater<double>> free;
     for (int i = 0; i < NS_SLOTS; i++) free.push(0.0);
@@ -901,9 +977,10 @@ double ns_plan_time(const std::vector<NsMat>& mats, int kind, int shape, int len
 
 // The order of one list: runs of neighbouring tiles of a matrix go to the XCD with the least work so far, the costly runs first;
 // the XCDs' queues, long reductions first, are then dealt out in turn (workgroup i starts on XCD i % 8), mat = -1 filling the gaps.
-int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out, std::vector<NsWork>& joins, long& partial_bytes) {
+int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out, std::vector<NsWork>& joins, long& partial_bytes,
+             double& best) {
   int shape = 0, len = 1 << 30;
-  double best = -1.0;
+  best = -1.0;
   for (int s = 0; s < 2; s++)
     for (int l : ns_lens) {
       const double t = ns_plan_time(mats, kind, s, l);
@@ -978,13 +1055,15 @@ int ns_plan(int n, const long* at, const int* rows, const int* cols, const float
   }
   std::vector<NsWork> work[3], join[3];
   NsPlan h = {};
+  double time[3];
   for (int k = 0; k < 3; k++) {
     long bytes = 0;
-    h.shape[k] = ns_order(mats, k, work[k], join[k], bytes);
+    h.shape[k] = ns_order(mats, k, work[k], join[k], bytes, time[k]);
     h.works[k] = (int)work[k].size();
     h.joins[k] = (int)join[k].size();
     partials = bytes > partials ? bytes : partials;
   }
+  h.pairs = ns_pairs(time);
   h.magic = NS_MAGIC;
   h.partials = ws;
   h.ws_bytes = ws + partials;
@@ -1091,5 +1170,5 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   last.ema_rest = ema_rest;
   last.do_ema = do_ema;
   last.state = ema ? state : nullptr;
-  return ns_iterate(r, steps, a, b, c, NS_OUT_MUON, last, stream);
+  return ns_iterate(r, steps, a, b, c, NS_OUT_MUON, last, h->pairs && ns_bounded(steps, a, b, c, true), stream);
 }

@@ -66,10 +66,10 @@ def test_plan_layout_and_refusals():
     # every chunk, and every tile on and above the diagonal / of the long side, exactly once
     w = blob[:256].view(torch.int64).tolist()
     i32 = lambda lo, n: blob[lo:lo + 4 * n].view(torch.int32).tolist()                                # noqa: E731
-    n_mats, chunks, areas, *rest = i32(40, 12)
+    n_mats, chunks, areas, *rest = i32(40, 14)
     shapes, works, joins = rest[:3], rest[3:6], rest[6:9]
-    at_mats, at_chunks, at_areas = w[11:14]
-    at_works, at_joins = w[14:17], w[17:20]
+    at_mats, at_chunks, at_areas = w[12:15]
+    at_works, at_joins = w[15:18], w[18:21]
     up = lambda v, d: -(-v // d)                                                                      # noqa: E731
     sides = [(32 * up(min(r, c), 32), 32 * up(max(r, c), 32)) for _, r, c in mats]
     ck = i32(at_chunks, 2 * chunks)
