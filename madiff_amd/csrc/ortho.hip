@@ -115,6 +115,9 @@ __device__ __forceinline__ size_t ns_chunk(int r, int k, int plane, int kblocks)
 }
 
 __device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) {      // v already scaled
+  // v as ONE fp32 number: contracted into the product it came from, hi was formed twice, once rounded from the exact product and
+  // once from its fp32 rounding, and where those two differ lo belonged to the other one (an error of 2^-11, one value in thousands)
+  asm("" : "+v"(v));
   hi = (_Float16)v;
   lo = (_Float16)(v - (float)hi);
 }

@@ -62,7 +62,8 @@ def _grad(shape, seed, rank=None, scale=1e-3, noise=0.1):
 
 
 SHAPES = [(1, 1), (1, 5), (7, 1), (2, 3), (16, 128), (31, 33), (127, 129), (128, 128), (129, 128), (128, 640), (130, 1000), (700, 100),
-          (333, 1001), (1024, 256), (257, 511), (512, 2560), (5, 20011), (1100, 1100)]
+          (333, 1001), (1024, 256), (257, 511), (512, 2560), (5, 20011), (1100, 1100),
+          (32, 1216), (1248, 30), (64, 512), (64, 513), (128, 192), (190, 127), (97, 224), (96, 290), (128, 256)]
 
 
 @pytest.mark.parametrize("t", list(TYPES))
