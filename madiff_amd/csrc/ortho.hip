@@ -709,6 +709,236 @@ __global__ __launch_bounds__(64) void ns_join_kernel(NsGroup grp, NsProduct q, N
   }
 }
 
+// ------------------------------------------------------------------------------------------------ one workgroup a matrix
+// A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything: by launches
+// a 16 x 128 matrix took 84 us, next to none of it work; here it takes 26 (64 x 512: 69, 128 x 96: 51; by launches 84 to 92).
+// What bounds it is one CU's chain of dependent products, fifteen of them with a barrier or two each.  Sixteen waves deal the
+// 32 x 32 blocks of a product among them (no mirror images: the whole squares are computed); a product that overwrites what it
+// reads keeps its blocks in registers until everybody has read.
+#define NS_SMALL_LDS 163840
+#define NS_SMALL_BLOCKS 3          // of X a wave: 4 sp lp + 4 sp^2 <= NS_SMALL_LDS leaves at most 39 of them
+
+template <int BYTES, bool BF16>
+__global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__ src, void* __restrict__ dst, NsMat one, long stride,
+                                                       int steps, float a, float b, float c, float eps) {
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[BYTES == NS_SMALL_LDS ? BYTES - 128 : BYTES];
+  __shared__ double part[16];
+  const NsMat& M = one;
+  const long at0 = (long)blockIdx.x * stride, n = (long)M.rows * M.cols;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 31, fh = lane >> 5, sb = M.sp >> 5, lb = M.lp >> 5, skb = M.sp >> 4, lkb = M.lp >> 4;
+  unsigned char *X = smem, *S = smem + 4 * M.sp * M.lp;
+  // X0: eight columns of X an item, at most five a lane, read once and kept while the norm is put together
+  constexpr int ITEMS = (NS_SMALL_LDS / 4 / 8 + 1023) / 1024;
+  float v0[ITEMS][8];
+  double sum = 0.0;
+#pragma unroll
+  for (int u = 0; u < ITEMS; u++) {
+    const int item = tid + 1024 * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
+    const long e = M.tall ? at0 + (long)col * M.cols + row : at0 + (long)row * M.cols + col;
+    const bool in = row < M.s;
+    if (!M.tall && in && col + 8 <= M.l) {
+      if constexpr (BF16) {
+        bf16_t h[8];
+        __builtin_memcpy(h, (const bf16_t*)src + e, 16);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v0[u][k] = to_f32(h[k]);
+      } else {
+        __builtin_memcpy(v0[u], (const float*)src + e, 32);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const long ek = e + (M.tall ? (long)k * M.cols : k);
+        v0[u][k] = !in || col + k >= M.l ? 0.f : BF16 ? to_f32(((const bf16_t*)src)[ek]) : ((const float*)src)[ek];
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < ITEMS; u++)
+#pragma unroll
+    for (int k = 0; k < 8; k++) sum += (double)v0[u][k] * (double)v0[u][k];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < 16; w++) sum += part[w];
+  const double norm = sqrt(sum);
+  const float inv = (float)((double)NS_SCALE / (norm > (double)eps ? norm : (norm <= (double)eps ? (double)eps : norm)));
+#pragma unroll
+  for (int u = 0; u < ITEMS; u++) {
+    const int item = tid + 1024 * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
+    if (row >= M.sp) continue;
+    f16x8 h, l;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      _Float16 hh, ll;
+      ns_split(v0[u][k] * inv, hh, ll);
+      h[k] = hh;
+      l[k] = ll;
+    }
+    *(f16x8*)(X + ns_chunk(row, col, 0, lkb)) = h;
+    *(f16x8*)(X + ns_chunk(row, col, 1, lkb)) = l;
+  }
+  __syncthreads();
+  // hi and lo of the rows 32 i .. + 31, columns 16 k .. + 15 of a matrix, as an operand
+  auto rows_of = [&](const unsigned char* P, int kb, int i, int k, f16x8& h, f16x8& l) {
+    const unsigned char* p = P + ((2 * i + (fr >> 4)) * kb + k) * 1024 + (fr & 15) * 64 + ((fh ^ ((fr >> 2) & 3) ^ ((k & 1) << 1)) << 4);
+    h = *(const f16x8*)p;
+    l = *(const f16x8*)(smem + ((p - smem) ^ 32));
+  };
+  // the same of the columns 32 j .. + 31 of X, rows 16 k .. + 15 (transposing read)
+  auto columns_of = [&](int j, int k, f16x8& h, f16x8& l) {
+    const int tq = (lane & 15) >> 2, tp = lane & 3, odd = (lane >> 4) & 1;
+    const int o = (k * lkb + 2 * j + odd) * 1024 + (8 * fh + tq) * 64 + (((tp >> 1) ^ (2 * fh) ^ (2 * odd)) << 4) + 8 * (tp & 1);
+    const int o2 = (o + 256) ^ 16;
+    const s16x4 h0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + o)), h1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + o2));
+    const s16x4 l0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + (o ^ 32))), l1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + (o2 ^ 32)));
+    h = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7));
+    l = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  f32x16 acc[NS_SMALL_BLOCKS];
+  // kind 0: X X^T, 1: S S, 2: S X, steps k0 to k1; block number first + 16 u of the result.  The large and the small
+  // products go into sums of their own: one chain would be three latencies long a step.
+  struct Pair { f16x8 ah, al, bh, bl; };
+  auto product = [&](auto kind, auto most, int blocks, int cols, int first, int k0, int k1) __attribute__((always_inline)) {
+    constexpr int KIND = decltype(kind)::value, MOST = decltype(most)::value;
+    ns_unroll<MOST>([&](auto uu) __attribute__((always_inline)) {
+      constexpr int u = decltype(uu)::value;
+      const int id = first + 16 * u;
+      if (id >= blocks) return;
+      const int i = id / cols, j = id - i * cols;
+      auto load = [&](Pair& f, int k) __attribute__((always_inline)) {
+        rows_of(KIND == 0 ? X : S, KIND == 0 ? lkb : skb, i, k, f.ah, f.al);
+        if constexpr (KIND == 2) columns_of(j, k, f.bh, f.bl);
+        else rows_of(KIND == 0 ? X : S, KIND == 0 ? lkb : skb, j, k, f.bh, f.bl);
+      };
+      f32x16 low;
+#pragma unroll
+      for (int r = 0; r < 16; r++) low[r] = acc[u][r] = 0.f;
+      auto multiply = [&](const Pair& f) __attribute__((always_inline)) {
+        low = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.bl, f.ah, low, 0, 0, 0);
+        acc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.bh, f.ah, acc[u], 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.bh, f.al, low, 0, 0, 0);
+      };
+      Pair f0, f1;
+      if (k0 < k1) load(f0, k0);
+      for (int k = k0; k < k1; k += 2) {                     // the next step's operands are read under this one's products
+        if (k + 1 < k1) load(f1, k + 1);
+        multiply(f0);
+        if (k + 2 < k1) load(f0, k + 2);
+        if (k + 1 < k1) multiply(f1);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[u][r] += low[r];
+    });
+  };
+  // the lane's values of block u, 16-byte chunk by chunk (columns 32 j + 16 p + 8 fh ..): f(v[8], row, column, number)
+  auto each = [&](auto most, int blocks, int cols, int first, auto f) __attribute__((always_inline)) {
+    ns_unroll<2 * decltype(most)::value>([&](auto at) __attribute__((always_inline)) {
+      constexpr int u = decltype(at)::value / 2, p = decltype(at)::value % 2;
+      const int id = first + 16 * u;
+      if (id >= blocks) return;
+      const int i = id / cols, j = id - i * cols;
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float s0 = acc[u][8 * p + r], s1 = acc[u][8 * p + 4 + r];
+        const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(s0), __float_as_uint(s1), false, false);
+        v[r] = __uint_as_float(w[0]) * (1.f / NS_SCALE);
+        v[4 + r] = __uint_as_float(w[1]) * (1.f / NS_SCALE);
+      }
+      f(v, 32 * i + fr, 32 * j + 16 * p + 8 * fh, at);
+    });
+  };
+  auto store = [&](unsigned char* P, int kb, const float (&v)[8], int row, int col) {
+    f16x8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      _Float16 hh, ll;
+      ns_split(v[e], hh, ll);
+      h[e] = hh;
+      l[e] = ll;
+    }
+    *(f16x8*)(P + ns_chunk(row, col, 0, kb)) = h;
+    *(f16x8*)(P + ns_chunk(row, col, 1, kb)) = l;
+  };
+  auto add = [&](float (&v)[8], const unsigned char* P, int kb, int row, int col, float f) {
+    const f16x8 h = *(const f16x8*)(P + ns_chunk(row, col, 0, kb)), l = *(const f16x8*)(P + ns_chunk(row, col, 1, kb));
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += f * ((float)h[e] + (float)l[e]);
+  };
+  using K0 = std::integral_constant<int, 0>;
+  using K1 = std::integral_constant<int, 1>;
+  using K2 = std::integral_constant<int, 2>;
+  using N1 = std::integral_constant<int, 1>;                 // 16 blocks of a square at most
+  using NB = std::integral_constant<int, NS_SMALL_BLOCKS>;
+  const int slices = max(1, min(sb == 1 ? 8 : sb == 2 ? 4 : 1, lkb / 4));
+  for (int step = 0; step < steps; step++) {
+    // A = X X^T has few blocks and a long reduction: `slices` waves share a block, each adding its part to what the one before it
+    // left in the block's own place
+    const int nb = sb * sb, part_of = wave / nb, block = part_of < slices ? wave - part_of * nb : nb;
+    product(K0{}, N1{}, nb, sb, block, lkb * part_of / slices, lkb * (part_of + 1) / slices);
+    for (int t = 0; t + 1 < slices; t++) {
+      f32x4* mine = (f32x4*)(S + block * 4096) + lane;
+      if (block < nb && part_of == t)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; r++) v[r] = acc[0][4 * g + r];
+          mine[64 * g] = v;
+        }
+      __syncthreads();
+      if (block < nb && part_of == t + 1)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const f32x4 v = mine[64 * g];
+#pragma unroll
+          for (int r = 0; r < 4; r++) acc[0][4 * g + r] += v[r];
+        }
+      __syncthreads();
+    }
+    each(N1{}, part_of == slices - 1 ? nb : 0, sb, block, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) { store(S, skb, v, row, col); });
+    __syncthreads();
+    product(K1{}, N1{}, sb * sb, sb, wave, 0, skb);
+    // R = b A + c A A, kept in the accumulators' place until every wave has read A
+    float keep[2][8];
+    each(N1{}, sb * sb, sb, wave, [&](float (&v)[8], int row, int col, auto at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] *= c;
+      add(v, S, skb, row, col, b);
+#pragma unroll
+      for (int e = 0; e < 8; e++) keep[decltype(at)::value][e] = v[e];
+    });
+    __syncthreads();
+    each(N1{}, sb * sb, sb, wave, [&](float (&)[8], int row, int col, auto at) __attribute__((always_inline)) {
+      store(S, skb, keep[decltype(at)::value], row, col);
+    });
+    __syncthreads();
+    product(K2{}, NB{}, sb * lb, lb, wave, 0, skb);
+    __syncthreads();                                         // X has been read: a X is added from a block's own place
+    each(NB{}, sb * lb, lb, wave, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
+      add(v, X, lkb, row, col, a);
+      store(X, lkb, v, row, col);
+    });
+    __syncthreads();
+  }
+  // out of the split form (22 bits: a last rounding of 2^-23), along the user's rows
+  for (long e = tid; e < n; e += 1024) {
+    const int r = (int)(e / M.cols), cc = (int)(e - (long)r * M.cols), row = M.tall ? cc : r, col = M.tall ? r : cc;
+    const unsigned char* at = X + ns_chunk(row, col & ~7, 0, lkb) + (col & 7) * 2;
+    const float v = ((float)*(const _Float16*)at + (float)*(const _Float16*)(smem + ((at - smem) ^ 32))) * (1.f / NS_SCALE);
+    if constexpr (BF16) ((bf16_t*)dst)[at0 + e] = (bf16_t)v;
+    else ((float*)dst)[at0 + e] = v;
+  }
+}
+
+static inline long ns_small_bytes(const NsMat& m) { return 4L * m.sp * m.lp + 4L * m.sp * m.sp; }
+static inline bool ns_small(const NsMat& m) { return m.sp <= 128 && ns_small_bytes(m) <= NS_SMALL_LDS - 128; }
+
 // ------------------------------------------------------------------------------------------------ host
 struct NsPlan {                    // start of a plan; matrices and lists follow
   long magic, bytes, ws_bytes, need, partials;       // need: elements the flat buffers must have
@@ -882,8 +1112,17 @@ static bool ns_bounded(int steps, float a, float b, float c, bool pairs) {
   return true;
 }
 
+// the same, remembered per thread for the last polynomial: walking the orbits takes longer than a small call
+static bool ns_fits(int steps, float a, float b, float c, bool pairs) {
+  struct Last { int steps; float a, b, c; bool fits; };
+  static thread_local Last last[2] = {{-1, 0.f, 0.f, 0.f, false}, {-1, 0.f, 0.f, 0.f, false}};
+  Last& l = last[pairs];
+  if (l.steps != steps || l.a != a || l.b != b || l.c != c) l = {steps, a, b, c, ns_bounded(steps, a, b, c, pairs)};
+  return l.fits;
+}
+
 extern "C" int madiff_ortho_check(int steps, float a, float b, float c, float eps) {
-  return steps >= 1 && steps <= 64 && eps > 0.f && eps < 1e30f && ns_bounded(steps, a, b, c, false) ? 0 : -1;
+  return steps >= 1 && steps <= 64 && eps > 0.f && eps < 1e30f && ns_fits(steps, a, b, c, false) ? 0 : -1;
 }
 
 // Everything about a call on `batch` equal matrices but its pointers
@@ -900,6 +1139,10 @@ static int ns_uniform(int batch, int rows, int cols, NsRun& r, long& ws_bytes) {
   r.n_chunks = batch * m.parts;
   r.per_areas = (int)areas;
   r.n_areas = batch * (int)areas;
+  if (ns_small(m)) {               // everything in LDS
+    ws_bytes = 0;
+    return 0;
+  }
   long slots = 0;
   double time[3];
   for (int k = 0; k < 3; k++) {
@@ -930,7 +1173,19 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
       madiff_ortho_check(steps, a, b, c, eps))
     return -1;
   if (batch == 0) return 0;
-  if (!src || !dst || !ws || ws_bytes < need || ((size_t)ws & 255)) return -1;
+  if (!src || !dst || (need > 0 && (!ws || ws_bytes < need || ((size_t)ws & 255)))) return -1;
+  const NsMat& m = r.grp.one;
+  if (ns_small(m)) {
+#define NS_GO(BYTES, BF16)                                                                                                        \
+  hipLaunchKernelGGL((ns_small_kernel<BYTES, BF16>), dim3(batch), dim3(1024), 0, stream, src, dst, m, r.grp.at_stride, steps, a, b, c, \
+                     eps)
+    const bool tiny = ns_small_bytes(m) <= 32768;             // several workgroups a CU
+    if (dtype == MADIFF_BF16) { if (tiny) NS_GO(32768, true); else NS_GO(NS_SMALL_LDS, true); }
+    else { if (tiny) NS_GO(32768, false); else NS_GO(NS_SMALL_LDS, false); }
+#undef NS_GO
+    MADIFF_CHECK_LAUNCH();
+    return 0;
+  }
   r.grp.ws = (unsigned char*)ws;
   NsSource q = {};
   q.src = src;
@@ -940,7 +1195,7 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
   MADIFF_CHECK_LAUNCH();
   NsProduct last = {};
   last.dst = dst;
-  const bool pairs = dtype == MADIFF_BF16 && r.pairs && ns_bounded(steps, a, b, c, true);
+  const bool pairs = dtype == MADIFF_BF16 && r.pairs && ns_fits(steps, a, b, c, true);
   return ns_iterate(r, steps, a, b, c, dtype == MADIFF_BF16 ? NS_OUT_BF16 : NS_OUT_F32, last, pairs, stream);
 }
 
@@ -1173,5 +1428,5 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   last.ema_rest = ema_rest;
   last.do_ema = do_ema;
   last.state = ema ? state : nullptr;
-  return ns_iterate(r, steps, a, b, c, NS_OUT_MUON, last, h->pairs && ns_bounded(steps, a, b, c, true), stream);
+  return ns_iterate(r, steps, a, b, c, NS_OUT_MUON, last, h->pairs && ns_fits(steps, a, b, c, true), stream);
 }

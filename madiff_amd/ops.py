@@ -1783,17 +1783,17 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
         raise ValueError(f"orthogonalize: matrices of {rows} x {cols} are out of range (shorter side up to 16384, longer up to "
                          "4194304)")
     dt, es = (lib.BF16 if x.dtype == torch.bfloat16 else lib.F32), x.element_size()
-    most = max(1, min(batch, ORTHO_WS_BYTES // need.value, ORTHO_MAX_BATCH))          # matrices a call
+    most = max(1, min(batch, ORTHO_WS_BYTES // max(need.value, 1), ORTHO_MAX_BATCH))          # matrices a call
     while lib._lib.madiff_ortho_ws(most, rows, cols, ctypes.byref(need)) != 0:
         most = (most + 1) // 2
     for lo in range(0, batch, most):
         n = min(most, batch - lo)
         if n != most:
             lib.call("madiff_ortho_ws", n, rows, cols, ctypes.byref(need))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)  # (stream-ordered, and private to a captured graph)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None   # (private to a captured graph)
         at = lo * rows * cols * es
         _launch(x, lambda st: lib.call("madiff_orthogonalize", dt, x.data_ptr() + at, out.data_ptr() + at, n, rows, cols, *args,
-                                       ws.data_ptr(), need.value, st))
+                                       _p(ws), need.value, st))
     return out
 
 

@@ -26,12 +26,13 @@ def test_c_refusals():
                 (5, 16.0, 0.0, 0.0, 1e-7), (5, 4.0, -4.0, 2.5, 1e-7)):
         assert L.madiff_ortho_check(*bad) == -1, bad
     need = C.c_long()
-    assert L.madiff_ortho_ws(3, 100, 200, C.byref(need)) == 0 and need.value > 0 and need.value % 256 == 0
+    assert L.madiff_ortho_ws(3, 100, 800, C.byref(need)) == 0 and need.value > 0 and need.value % 256 == 0
+    assert L.madiff_ortho_ws(3, 50, 200, C.byref(need)) == 0 and need.value == 0      # whole in LDS: no workspace
     for bad in ((-1, 4, 4), (1, 0, 4), (1, 4, 0), (1, 16385, 16385), (1, 2, (1 << 22) + 1), (1 << 30, 128, 128)):
         assert L.madiff_ortho_ws(*bad, C.byref(need)) == -1, bad
-    L.madiff_ortho_ws(3, 100, 200, C.byref(need))
+    L.madiff_ortho_ws(3, 100, 800, C.byref(need))
     p = 1 << 20
-    ok = [1, p, p, 3, 100, 200, 5, *ns, 1e-7, p, need.value, None]
+    ok = [1, p, p, 3, 100, 800, 5, *ns, 1e-7, p, need.value, None]
     for at, bad in ((0, 2), (1, None), (2, None), (3, -1), (4, 0), (5, 0), (6, 0), (10, 0.0), (11, None), (11, p + 16), (12, need.value - 1)):
         args = list(ok)
         args[at] = bad
