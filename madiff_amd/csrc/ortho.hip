@@ -1388,7 +1388,7 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
                                 int steps, float a, float b, float c, float eps, void* ws, long ws_bytes, hipStream_t stream) {
   const NsPlan* h = (const NsPlan*)plan;
   if (!h || h->magic != NS_MAGIC || !plan_device || !p || !g || !m || n < h->need || !ws || ws_bytes < h->ws_bytes ||
-      ((size_t)ws & 255) || madiff_ortho_check(steps, a, b, c, eps) || do_ema < 0 || do_ema > 2 || (!ema && (do_ema && !state)) ||
+      ((size_t)ws & 255) || madiff_ortho_check(steps, a, b, c, eps) || do_ema < 0 || do_ema > 2 || (!ema && do_ema) ||
       !(momentum >= 0.f && momentum < 1.f))
     return -1;
   const unsigned char* dev = (const unsigned char*)plan_device;

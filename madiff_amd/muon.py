@@ -71,18 +71,19 @@ class MuonPlan:
              shadow: Optional[torch.Tensor] = None, grad_scale: float = 1.0, zero_grad: bool = False, steps: int = 5,
              coefficients: Sequence[float] = ops.NEWTON_SCHULZ, eps: float = 1e-7, state: Optional[torch.Tensor] = None) -> None:
         """One step, in place, on the current stream: p, g, m (and ema) flat float32, shadow bfloat16.  do_ema: 0 none, 1 lerp
-        with ema_beta (the default where ema is given), 2 copy; state (int32[2] on the GPU): the mode is state[1] instead.
+        with ema_beta (the default where ema is given), 2 copy; state (int32[2] on the GPU): the mode is state[1] instead
+        (none without ema).
         zero_grad: clear g as it is read.  Elements outside the plan's matrices are not touched."""
         ptrs = [self._check(k, t) for k, t in (("p", p), ("g", g), ("m", m))]
         pe = None if ema is None else self._check("ema", ema)
         ps = None if shadow is None else self._check("shadow", shadow, torch.bfloat16)
-        bufs = [t for t in (p, g, m, ema) if t is not None]
-        if len({t.data_ptr() for t in bufs}) != len(bufs):
-            raise ValueError("MuonPlan.step: p, g, m and ema have to be different buffers")
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (p, g, m, ema, shadow) if t is not None)
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("MuonPlan.step: p, g, m, ema and shadow must not overlap")
         if state is not None and (state.device != self.device or state.dtype != torch.int32 or state.numel() < 2):
             raise ValueError(f"MuonPlan.step: state has to be an int32[2] on {self.device}")
         do_ema = (0 if ema is None else 1) if do_ema is None else int(do_ema)
-        if do_ema not in (0, 1, 2) or (do_ema and ema is None and state is None):
+        if do_ema not in (0, 1, 2) or (do_ema and ema is None):
             raise ValueError(f"MuonPlan.step: do_ema has to be 0, 1 or 2, and 0 without ema, not {do_ema}")
         lr, momentum, weight_decay, ema_beta = float(lr), float(momentum), float(weight_decay), float(ema_beta)
         if not 0.0 <= momentum < 1.0:

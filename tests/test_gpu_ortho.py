@@ -291,10 +291,12 @@ def test_refusals_on_the_gpu():
         ops.orthogonalize(x.clone().requires_grad_(True))
     plan = MuonPlan([(0, 4, 5)], DEV)
     p, g, m = (torch.zeros(20, device=DEV) for _ in range(3))
+    both = torch.zeros(40, device=DEV)
     for args, kw in (((p[:19], g, m), {}), ((p, g.double(), m), {}), ((p, g, p), {}), ((p, g, m), dict(do_ema=1)),
                      ((p, g, m), dict(momentum=1.0)), ((p, g, m), dict(steps=0)), ((p.cpu(), g, m), {}),
                      ((p, g, m), dict(shadow=torch.zeros(20, device=DEV))), ((p, g, m), dict(ema=p)),
-                     ((p, torch.zeros(40, device=DEV)[::2], m), {}), ((p, g, m), dict(ema=g.clone(), state=torch.zeros(1, device=DEV)))):
+                     ((p, torch.zeros(40, device=DEV)[::2], m), {}), ((both[:20], both[10:], m), {}), ((both, both[20:], m), {}),
+                     ((p, g, m), dict(do_ema=1, state=torch.zeros(2, device=DEV, dtype=torch.int32))), ((p, g, m), dict(ema=g.clone(), state=torch.zeros(1, device=DEV)))):
         with pytest.raises(ValueError):
             plan.step(*args, lr=0.1, **kw)
     with pytest.raises(ValueError):

@@ -105,3 +105,8 @@ def test_plan_layout_and_refusals():
         args = list(ok)
         args[at] = v
         assert L.madiff_muon_step(*args) == -1, (at, v)
+    args = list(ok)                                  # an EMA mode without a buffer, with and without a mode on the device
+    args[5] = None
+    assert L.madiff_muon_step(*args) == -1
+    args[18] = p
+    assert L.madiff_muon_step(*args) == -1
