@@ -18,12 +18,13 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Dict, List, Optional
+from typing import Callable, Dict, List, Optional
 
 import torch
 import torch.distributed as dist
 
 from . import lib, ops
+from .muon import MuonPlan
 
 
 class FlatAdamEMA:
@@ -104,7 +105,7 @@ class FlatAdamEMA:
                     seen.add(id(q))
                     order.append(q)
         name_of = {id(p): n for n, p in named}
-        self.params = order
+        self.params = order = self._layout_order(order, name_of, known)
         self.names = [name_of[id(p)] for p in order]
         offs, total, geoms = [], 0, []
         for p in self.params:
@@ -403,12 +404,7 @@ class FlatAdamEMA:
         if self.use_hip:
             cur = torch.cuda.current_stream()
             if not early:                            # nothing was issued during backward: one launch over everything
-                lib.call("madiff_adam_ema", self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.flat_m.data_ptr(),
-                         self.flat_v.data_ptr(), None if self.flat_ema is None else self.flat_ema.data_ptr(), self.total,
-                         self.lr, b1, b2, self.eps, 1 - b1 ** (self.step_count + 1),
-                         math.sqrt(1 - b2 ** (self.step_count + 1)), scale, do_ema, self.ema_decay,
-                         None if device_state is None else device_state.data_ptr(),
-                         self.flat_p16.data_ptr(), 1, cur.cuda_stream)
+                self._update(do_ema, device_state, scale, cur)
             else:                                    # the remaining slices, then advance the device-side counter once
                 for b in self.buckets:
                     if not b.get("opt"):
@@ -423,18 +419,40 @@ class FlatAdamEMA:
             ops.params_changed(by_optimizer=True)
         else:   # host arithmetic for the gloo/CPU tests of the data-parallel machinery only
             self.step_count += 1
-            bc1 = 1 - b1 ** self.step_count
-            bc2s = math.sqrt(1 - b2 ** self.step_count)
             with torch.no_grad():
-                g = self.flat_g * scale
-                self.flat_m.mul_(b1).add_(g, alpha=1 - b1)
-                self.flat_v.mul_(b2).addcmul_(g, g, value=1 - b2)
-                denom = (self.flat_v.sqrt() / bc2s).add_(self.eps)
-                self.flat_p.addcdiv_(self.flat_m, denom, value=-self.lr / bc1)
-                if do_ema == 1:
-                    self.flat_ema.mul_(self.ema_decay).add_(self.flat_p, alpha=1 - self.ema_decay)
-                elif do_ema == 2:
-                    self.flat_ema.copy_(self.flat_p)
+                self._update_host(do_ema, scale)
+
+    def _layout_order(self, order, name_of, known):
+        """The order of the parameters in the flat buffers; members of a fused group stay next to each other."""
+        return order
+
+    def _update(self, do_ema, device_state, scale, stream, n: Optional[int] = None):
+        """The whole update in one launch, over the first n elements (default: all)."""
+        b1, b2 = self.betas
+        lib.call("madiff_adam_ema", self.flat_p.data_ptr(), self.flat_g.data_ptr(), self.flat_m.data_ptr(),
+                 self.flat_v.data_ptr(), None if self.flat_ema is None else self.flat_ema.data_ptr(),
+                 self.total if n is None else n, self.lr, b1, b2, self.eps, 1 - b1 ** (self.step_count + 1),
+                 math.sqrt(1 - b2 ** (self.step_count + 1)), scale, do_ema, self.ema_decay,
+                 None if device_state is None else device_state.data_ptr(),
+                 self.flat_p16.data_ptr(), 1, stream.cuda_stream)
+
+    def _update_host(self, do_ema, scale, n: Optional[int] = None):
+        b1, b2 = self.betas
+        bc1 = 1 - b1 ** self.step_count
+        bc2s = math.sqrt(1 - b2 ** self.step_count)
+        p, m, v = self.flat_p[:n], self.flat_m[:n], self.flat_v[:n]
+        g = self.flat_g[:n] * scale
+        m.mul_(b1).add_(g, alpha=1 - b1)
+        v.mul_(b2).addcmul_(g, g, value=1 - b2)
+        denom = (v.sqrt() / bc2s).add_(self.eps)
+        p.addcdiv_(m, denom, value=-self.lr / bc1)
+        self._ema_host(do_ema, 0, n)
+
+    def _ema_host(self, do_ema, lo: int, hi: Optional[int]):
+        if do_ema == 1:
+            self.flat_ema[lo:hi].mul_(self.ema_decay).add_(self.flat_p[lo:hi], alpha=1 - self.ema_decay)
+        elif do_ema == 2:
+            self.flat_ema[lo:hi].copy_(self.flat_p[lo:hi])
 
     def broadcast_parameters(self, src: int = 0):
         """Make every rank start from rank `src`'s weights (the reference has one process; DP needs this once)."""
@@ -446,6 +464,106 @@ class FlatAdamEMA:
             for p in self.ema_module.parameters():
                 dist.broadcast(p.data, src=src, group=self.pg)
         ops.params_changed()
+
+
+class FlatMuonEMA(FlatAdamEMA):
+    """Muon for the weight matrices, Adam for the rest (gains, shifts, biases, embeddings): the step of muon.MuonPlan over the
+    flat buffers, next to the fused Adam/EMA launch.  Not in the reference, whose only optimizer is Adam
+    (diffuser/utils/training.py:109).
+
+    A matrix is a parameter of two or more axes, not the weight of an nn.Embedding, with more than one row and column as
+    [out channels, in channels * taps]; select(name, parameter), where given, picks among those.  Members of a fused group
+    (q/k/v, the time MLPs) are orthogonalised one by one and go to Adam only together.  The update of a matrix is
+    lr * 0.2 * sqrt(max(rows, columns)) times the orthogonalised momentum: its elements then have about the size that Adam's
+    have, so one lr (the reference's) serves both.
+
+    The rest lies in front of the matrices in the flat buffers: each optimizer has one contiguous range, and the buckets of
+    the data-parallel all-reduce, cut from the end, still complete in backward's order.  No part of the step is issued under
+    backward: the matrices' products need the whole chip and their shared tables all matrices at once."""
+
+    def __init__(self, module, ema_module=None, lr: float = 2e-4, *, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, ns_steps: int = 5, select: Optional[Callable[[str, torch.nn.Parameter], bool]] = None,
+                 **kwargs):
+        super().__init__(module, ema_module, lr=lr, **kwargs)
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"FlatMuonEMA: momentum has to be in [0, 1), not {momentum}")
+        if not (weight_decay >= 0.0 and math.isfinite(weight_decay)):
+            raise ValueError(f"FlatMuonEMA: weight_decay has to be finite and not negative, not {weight_decay}")
+        ops._check_newton_schulz("FlatMuonEMA", ns_steps, ops.NEWTON_SCHULZ, 1e-7)
+        self.momentum, self.nesterov, self.weight_decay, self.ns_steps, self.select = momentum, nesterov, weight_decay, ns_steps, select
+        self.overlap = False
+        self.plan: Optional[MuonPlan] = None
+        self.matrices: List[str] = []              # their names
+        self.split = 0                             # first element of the matrices
+
+    def _layout_order(self, order, name_of, known):
+        embedded = {id(m.weight) for m in self.module.modules() if isinstance(m, torch.nn.Embedding)}
+        self._transposed = {id(m.weight) for m in self.module.modules()
+                            if isinstance(m, (torch.nn.ConvTranspose1d, torch.nn.ConvTranspose2d, torch.nn.ConvTranspose3d))}
+
+        def matrix(p):
+            if p.dim() < 2 or id(p) in embedded or (self.use_hip and id(p) in self._transposed and id(p) not in known):
+                return False
+            rows = p.shape[1 if id(p) in self._transposed else 0]
+            return 1 < rows < p.numel() and (self.select is None or bool(self.select(name_of[id(p)], p)))
+
+        chosen = {id(p) for p in order if matrix(p)}
+        for p in order:                            # a fused group is one piece of the buffers
+            group = known[id(p)][2] if id(p) in known else ()
+            if not all(i in chosen for i in group if i in name_of):
+                chosen.difference_update(group)
+        self._chosen = chosen
+        return [p for p in order if id(p) not in chosen] + [p for p in order if id(p) in chosen]
+
+    def _materialise(self):
+        super()._materialise()
+        mats, scales = [], []
+        self.split = self.total
+        for n, p, o, geom in zip(self.names, self.params, self.offsets, self.geoms):
+            if id(p) not in self._chosen:
+                continue
+            if geom is not None:
+                _, taps, O, I, ipad = geom
+                rows, cols, real = O, taps * ipad, taps * I
+            else:
+                rows = p.shape[1 if id(p) in self._transposed else 0]
+                cols = real = p.numel() // rows
+            if not mats:
+                self.split = o
+            self.matrices.append(n)
+            mats.append((o, rows, cols))
+            scales.append(0.2 * math.sqrt(max(rows, real)))
+        self._mats, self._scales = mats, scales
+        if self.use_hip and mats:
+            self.plan = MuonPlan(mats, device=self.flat_p.device, scales=scales)
+        self.flat_v = self.flat_v[:self.split].clone()      # second moments: Adam's range only
+
+    def _update(self, do_ema, device_state, scale, stream, n=None):
+        if self.plan is not None:                  # (before Adam, whose launch advances the step counter in device_state)
+            ops._timed("muon_step", 0.0, lambda: self.plan.step(
+                self.flat_p, self.flat_g, self.flat_m, lr=self.lr, momentum=self.momentum, nesterov=self.nesterov,
+                weight_decay=self.weight_decay, ema=self.flat_ema, ema_beta=self.ema_decay, do_ema=int(do_ema),
+                shadow=self.flat_p16, grad_scale=scale, zero_grad=True, steps=self.ns_steps, state=device_state), stream=stream)
+        super()._update(do_ema, device_state, scale, stream, self.split)
+
+    def _update_host(self, do_ema, scale, n=None):
+        super()._update_host(do_ema, scale, self.split)
+        a, b, c = ops.NEWTON_SCHULZ
+        for p, (o, rows, cols), s in zip(self.params[-len(self._mats):] if self._mats else (), self._mats, self._scales):
+            g, m, w = (f[o:o + rows * cols].view_as(p) for f in (self.flat_g, self.flat_m, self.flat_p))
+            m.mul_(self.momentum).add_(g, alpha=(1 - self.momentum) * scale)
+            u = m * self.momentum + g * ((1 - self.momentum) * scale) if self.nesterov else m
+            if id(p) in self._transposed:
+                u, w = u.transpose(0, 1), w.transpose(0, 1)
+            x = u.reshape(rows, cols)
+            x = x.T if rows > cols else x
+            x = x / (x.norm() + 1e-7)
+            for _ in range(self.ns_steps):
+                r = x @ x.T
+                x = a * x + (b * r + c * (r @ r)) @ x
+            x = x.T if rows > cols else x
+            w.mul_(1 - self.lr * self.weight_decay).sub_(x.reshape(w.shape), alpha=self.lr * s)
+        self._ema_host(do_ema, self.split, None)
 
 
 FOLD_MICRO_BATCHES = os.environ.get("MADIFF_FOLD_MICRO", "1") != "0"

@@ -29,7 +29,7 @@ import torch.distributed as dist
 
 from . import ops
 from .host import batch_to_device
-from .trainer import FlatAdamEMA, GraphedTrainStep, train_step
+from .trainer import FlatAdamEMA, FlatMuonEMA, GraphedTrainStep, train_step
 
 try:                                            # the reference logs through ml_logger (absent from this image)
     from ml_logger import logger as _ml_logger  # type: ignore
@@ -120,17 +120,24 @@ class DevicePrefetcher:
         return batch
 
 
+OPTIMIZERS = {"adam": FlatAdamEMA, "muon": FlatMuonEMA}
+
+
 class Trainer(object):
     def __init__(self, diffusion_model, dataset, renderer, ema_decay=0.995, train_batch_size=32, train_lr=2e-5,
                  gradient_accumulate_every=2, step_start_ema=2000, update_ema_every=10, log_freq=100, sample_freq=1000,
                  save_freq=1000, label_freq=100000, eval_freq=100000, save_parallel=False, n_reference=8, bucket=None,
                  train_device="cuda", save_checkpoints=False, use_graph: Optional[bool] = None, bucket_mb: float = 64.0,
-                 shuffle: bool = True, seed: int = 0, allow_eager_fallback: Optional[bool] = None):
+                 shuffle: bool = True, seed: int = 0, allow_eager_fallback: Optional[bool] = None, optimizer: str = "adam",
+                 optimizer_kwargs: Optional[dict] = None):
         """Reference arguments (training.py:43-64) plus: use_graph (None = replay the step from a hipGraph on a GPU),
-        bucket_mb (gradient bucket size of the data-parallel all-reduce / optimizer slices), shuffle, seed.
+        bucket_mb (gradient bucket size of the data-parallel all-reduce / optimizer slices), shuffle, seed, optimizer ("adam",
+        the reference's, or "muon" = FlatMuonEMA) and optimizer_kwargs (further arguments of its constructor).
         The reference's DataLoader keeps the smaller last batch of an epoch; a replayed graph (and equal work per
         rank) needs fixed shapes, so that batch is dropped when use_graph is on or under data parallelism."""
         super().__init__()
+        if optimizer not in OPTIMIZERS:
+            raise ValueError(f"Trainer: optimizer has to be one of {sorted(OPTIMIZERS)}, not {optimizer!r}")
         self.model = diffusion_model
         self.ema = EMA(ema_decay)
         self.ema_model = copy.deepcopy(self.model)
@@ -164,7 +171,8 @@ class Trainer(object):
                 self.dataset, batch_size=1, num_workers=0, shuffle=True, pin_memory=on_gpu))
         self.renderer = renderer
         # Adam(lr, torch defaults) + EMA over the same parameters as the reference's torch.optim.Adam (training.py:109)
-        self.optimizer = FlatAdamEMA(diffusion_model, self.ema_model, lr=train_lr, ema_decay=ema_decay, bucket_mb=bucket_mb)
+        self.optimizer = OPTIMIZERS[optimizer](diffusion_model, self.ema_model, lr=train_lr, ema_decay=ema_decay,
+                                               bucket_mb=bucket_mb, **(optimizer_kwargs or {}))
         self.optimizer.broadcast_parameters(0)
         self.bucket = bucket
         self.n_reference = n_reference
