@@ -3,10 +3,14 @@
 //   mu = mean_c x,  v = mean_c (x - mu)^2,  r = (v + eps)^-1/2,  h = (x - mu) r,  y = h w + b
 //   g = dy w,  dx = r (g - mean_c g - h mean_c(g h)),  dw = sum_rows dy h,  db = sum_rows dy
 //
-// Bandwidth-bound: forward reads x and writes y once, backward reads x and dy and writes dx once.  A row lives in the
-// registers of a group of lanes: 8..64 lanes of one wave while R <= 4 vectors of 16 bytes a lane hold it, else a
-// workgroup of 256 or 1024 lanes.  Groups stride over the rows with their share of w and b in registers (read from L2
-// for every row they would cost four times the bf16 row itself) and with the next row's loads in flight.  The variance
+// Bandwidth-bound: forward reads x and writes y once, backward reads x and dy and writes dx once.  A row lives in the registers of
+// a group of lanes, 16 elements (or fewer) each: 8..64 lanes of one wave, or a workgroup of 128..1024; only above 16384 columns a
+// lane has 32.  (32 bf16 elements a lane in one wave, or 256 lanes for rows up to 8192 columns with one workgroup a CU: too few
+// waves and loads in flight; 65536 x 2048 backward took 460 us, now 173; 16384 x 8192 418, now 178.)  Groups stride over the rows
+// with their share of w and b in registers (read from L2 for every row they would cost four times the bf16 row itself) and with
+// the next row's loads in flight.  Measured with cold caches, where a 4 GiB copy reaches 4.6 TB/s: bf16 262144 x 1024 forward 230 us
+// (4.7 TB/s) and backward 316 (5.1), 32768 x 4096 128 and 168 (4.2, 4.8), 4093 x 16384 74 and 97 (3.7, 4.2); fp32 65536 x 1024 116
+// and 157 (4.6, 5.1).  The widest rows, 2000 x 32768 bf16: 92 and 259 (2.9, 1.5; dw and db fill the registers).  The variance
 // is the second pass over the registers, not E[x^2] - mu^2.  All arithmetic is fp32; the only rounding to fewer bits is
 // that of y and dx to the storage type of x.
 // dw / db: every lane sums its own columns over the rows of its group in fp32 registers, a workgroup's groups meet in LDS,
@@ -14,9 +18,17 @@
 // call gives the same bits.
 #include "common.h"
 
-template <typename T> struct LnVec { static constexpr int N = 16 / sizeof(T); T v[N]; };
+// 16 bytes of a row as they lie in memory: four registers whatever the type (as eight bf16 values they took eight)
+template <typename T> struct LnVec {
+  static constexpr int N = 16 / sizeof(T);
+  uint32_t u[4];
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (N == 4) return __uint_as_float(u[e]);
+    else return __uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
+  }
+};
 
-// 16 bytes from an address that is only element-aligned (rows of odd widths begin anywhere; the hardware takes it)
+// from an address that is only element-aligned (rows of odd widths begin anywhere; the hardware takes it)
 template <typename T> __device__ __forceinline__ LnVec<T> ln_load(const T* p) {
   LnVec<T> r;
   __builtin_memcpy(&r, p, 16);
@@ -25,16 +37,26 @@ template <typename T> __device__ __forceinline__ LnVec<T> ln_load(const T* p) {
 template <typename T> __device__ __forceinline__ LnVec<T> ln_load_part(const T* p, int n) {   // n elements, zeros behind
   LnVec<T> r;
 #pragma unroll
-  for (int e = 0; e < LnVec<T>::N; e++) r.v[e] = e < n ? p[e] : from_f32<T>(0.f);
+  for (int k = 0; k < 4; k++) {
+    r.u[k] = 0;
+    if constexpr (sizeof(T) == 4) {
+      if (k < n) __builtin_memcpy(&r.u[k], p + k, 4);
+    } else {
+      uint16_t lo = 0, hi = 0;
+      if (2 * k < n) __builtin_memcpy(&lo, p + 2 * k, 2);
+      if (2 * k + 1 < n) __builtin_memcpy(&hi, p + 2 * k + 1, 2);
+      r.u[k] = lo | (uint32_t)hi << 16;
+    }
+  }
   return r;
 }
-// one lane's R vectors of a row: columns (l + i LPR) N .. + N
-template <typename T, int LPR, int R>
+// R vectors of a lane from its FROM-th on: columns (l + i LPR) N .. + N
+template <typename T, int LPR, int R, int FROM = 0>
 __device__ __forceinline__ void ln_row(LnVec<T> (&d)[R], const T* row, int l, int C) {
   constexpr int N = LnVec<T>::N;
 #pragma unroll
   for (int i = 0; i < R; i++) {
-    const int c = (l + i * LPR) * N;
+    const int c = (l + (FROM + i) * LPR) * N;
     if (c + N <= C) d[i] = ln_load(row + c);
     else d[i] = ln_load_part(row + (c < C ? c : 0), c < C ? C - c : 0);
   }
@@ -53,9 +75,9 @@ template <typename T>
 __device__ __forceinline__ void ln_put(T* row, const float (&y)[LnVec<T>::N], int c, int C) {
   constexpr int N = LnVec<T>::N;
   if (c + N <= C) {
-    LnVec<T> o;
+    T o[N];
 #pragma unroll
-    for (int e = 0; e < N; e++) o.v[e] = from_f32<T>(y[e]);
+    for (int e = 0; e < N; e++) o[e] = from_f32<T>(y[e]);
     __builtin_memcpy(row + c, &o, 16);
   } else if (c < C) {
 #pragma unroll
@@ -64,15 +86,35 @@ __device__ __forceinline__ void ln_put(T* row, const float (&y)[LnVec<T>::N], in
   }
 }
 
-// Sum of K values over the LPR lanes of a group.  Within a wave by shuffles; across the waves of a workgroup through LDS,
-// in wave order.  `slot` alternates from call to call, so that one barrier a call is enough: the values of a call are
-// overwritten two calls later, behind the barrier of the call between.
+// Sum over LPR = 2..64 neighbouring lanes, the same bits in each of them: by DPP within rows of 16 lanes, then by swaps of rows
+// and halves.  (Through LDS the six dependent shuffles of a row took longer than its arithmetic.)
+template <int LPR> __device__ __forceinline__ float ln_lanes(float v) {
+#define LN_DPP(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
+  LN_DPP(0xB1);                            // lane ^ 1
+  if constexpr (LPR >= 4) LN_DPP(0x4E);    // lane ^ 2
+  if constexpr (LPR >= 8) LN_DPP(0x141);   // 7 - lane: the other four of eight
+  if constexpr (LPR >= 16) LN_DPP(0x140);  // 15 - lane: the other eight
+#undef LN_DPP
+  if constexpr (LPR >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const unsigned lo = r[0], hi = r[1];
+    v = __uint_as_float(lo) + __uint_as_float(hi);
+  }
+  if constexpr (LPR >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const unsigned lo = r[0], hi = r[1];
+    v = __uint_as_float(lo) + __uint_as_float(hi);
+  }
+  return v;
+}
+
+// Sum of K values over the LPR lanes of a group: within its waves, then across them through LDS.  `slot`
+// alternates from call to call, so that one barrier a call is enough: the values of a call are overwritten two calls later,
+// behind the barrier of the call between.
 template <int LPR, int K>
 __device__ __forceinline__ void ln_sum(float (&v)[K], float* lds, int& slot) {
 #pragma unroll
-  for (int k = 0; k < K; k++)
-#pragma unroll
-    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v[k] += __shfl_xor(v[k], o, 64);
+  for (int k = 0; k < K; k++) v[k] = ln_lanes<(LPR < 64 ? LPR : 64)>(v[k]);
   if constexpr (LPR > 64) {
     constexpr int W = LPR / 64;
     float* s = lds + slot * (K * W);
@@ -82,24 +124,20 @@ __device__ __forceinline__ void ln_sum(float (&v)[K], float* lds, int& slot) {
       for (int k = 0; k < K; k++) s[k * W + (threadIdx.x >> 6)] = v[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      v[k] = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; w++) v[k] += s[k * W + w];
-    }
+    for (int k = 0; k < K; k++) v[k] = ln_lanes<W>(s[k * W + (threadIdx.x & (W - 1))]);
   }
 }
 
 template <typename T, int LPR, int R>
-__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
+__global__ __launch_bounds__(LPR > 64 ? LPR : 256) void layer_norm_fwd_kernel(
     const T* __restrict__ x, long ldx, T* __restrict__ y, long ldy, const float* __restrict__ w, const float* __restrict__ b,
     float* __restrict__ mean_out, float* __restrict__ rstd_out, long rows, int C, int Cpad, float eps) {
-  constexpr int N = LnVec<T>::N, BLOCK = LPR > 256 ? LPR : 256, GPB = LPR > 64 ? 1 : BLOCK / LPR;
+  constexpr int N = LnVec<T>::N, BLOCK = LPR > 64 ? LPR : 256, GPB = LPR > 64 ? 1 : BLOCK / LPR;
   __shared__ float lds[LPR > 64 ? 2 * (LPR / 64) : 1];
-  const int l = threadIdx.x % LPR;
+  int l = threadIdx.x % LPR;
   const long g0 = (long)blockIdx.x * GPB + (GPB > 1 ? threadIdx.x / LPR : 0), gs = (long)gridDim.x * GPB;
   int slot = 0;
-  constexpr bool LEAN = LPR == 1024;     // 128 registers a lane: gains and shifts come from L2 row by row, no row is prefetched
+  constexpr bool LEAN = R * N > 16;      // 128 registers a lane: gains and shifts come from L2 row by row, no row is prefetched
   float wv[LEAN ? 1 : R][N], bv[LEAN ? 1 : R][N];
   if constexpr (!LEAN)
 #pragma unroll
@@ -111,6 +149,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
   if (!LEAN && g0 < rows) ln_row<T, LPR, R>(nx, x + g0 * ldx, l, C);
   const float inv = 1.f / (float)C;
   for (long r = g0; r < rows; r += gs) {
+    asm("" : "+v"(l));                   // (else every vector's addresses and tail tests stay in registers over all rows)
     const float *wr = w, *br = b;
     if constexpr (LEAN) {
       asm("" : "+s"(wr), "+s"(br));        // (not loop-invariant to the compiler: it would hold them in registers)
@@ -122,7 +161,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
     for (int i = 0; i < R; i++)
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        v[i][e] = to_f32(nx[i].v[e]);
+        v[i][e] = nx[i].at(e);
         s[0] += v[i][e];
       }
     if (!LEAN && r + gs < rows) ln_row<T, LPR, R>(nx, x + (r + gs) * ldx, l, C);
@@ -157,17 +196,22 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_fwd_kernel(
 
 // part: [gridDim.x, 2, C] column sums (dw then db) of the workgroup's rows; null = no parameter gradient wanted.
 template <typename T, int LPR, int R>
-__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
+// (bf16 up to 128 lanes: 128 registers, four waves a SIMD, for three spilled ones: 262144 x 1024 316 us, with 130 registers and three
+// waves 354.  fp32 would spill forty: 6151 x 777 21 us, held to 128 registers 37.)
+__global__ __launch_bounds__((LPR > 64 ? LPR : 256), (sizeof(T) == 2 && LPR <= 128 ? 4 : 1)) void layer_norm_bwd_kernel(
     const T* __restrict__ x, long ldx, const T* __restrict__ dy, long lddy, const float* __restrict__ w,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx, long lddx,
     float* __restrict__ part, long rows, int C, int Cpad) {
-  constexpr int N = LnVec<T>::N, BLOCK = LPR > 256 ? LPR : 256, GPB = LPR > 64 ? 1 : BLOCK / LPR;
+  constexpr int N = LnVec<T>::N, BLOCK = LPR > 64 ? LPR : 256, GPB = LPR > 64 ? 1 : BLOCK / LPR;
   constexpr int COLS = 64 * R * N;                           // columns a wave covers (LPR <= 64)
   __shared__ float lds[LPR > 64 ? 4 * (LPR / 64) : 3 * COLS];
-  const int l = threadIdx.x % LPR;
+  int l = threadIdx.x % LPR;
   const long g0 = (long)blockIdx.x * GPB + (GPB > 1 ? threadIdx.x / LPR : 0), gs = (long)gridDim.x * GPB;
   int slot = 0;
-  constexpr bool LEAN = LPR == 1024;     // 128 registers a lane: the row stays in its storage type, h and g are formed twice
+  // LEAN: 1024 lanes have 128 registers each.  h and g are formed twice, gains come from L2 row by row, no row is prefetched;
+  // KEEP: x waits in LDS, each lane's vectors for itself (no barrier).
+  constexpr bool LEAN = R * N > 16 || (LPR == 1024 && N == 4), KEEP = R * N > 16;
+  __shared__ LnVec<T> keep[KEEP ? R * LPR : 1];
   float wv[LEAN ? 1 : R][N], aw[R][N], ab[R][N];
 #pragma unroll
   for (int i = 0; i < R; i++) {
@@ -175,20 +219,33 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
 #pragma unroll
     for (int e = 0; e < N; e++) aw[i][e] = ab[i][e] = 0.f;
   }
-  LnVec<T> nx[R], nd[R];
+  LnVec<T> nx[KEEP ? R / 2 : R], nd[R];
   if (!LEAN && g0 < rows) {
-    ln_row<T, LPR, R>(nx, x + g0 * ldx, l, C);
+    ln_row<T, LPR, (KEEP ? R / 2 : R)>(nx, x + g0 * ldx, l, C);
     ln_row<T, LPR, R>(nd, dy + g0 * lddy, l, C);
   }
   const float inv = 1.f / (float)C;
   for (long r = g0; r < rows; r += gs) {
+    asm("" : "+v"(l));                   // (else every vector's addresses and tail tests stay in registers over all rows)
     const float mean = mean_in[r], rstd = rstd_in[r];
     const float* wr = w;
     if constexpr (LEAN) {
       asm("" : "+s"(wr));
-      ln_row<T, LPR, R>(nx, x + r * ldx, l, C);
+      if constexpr (KEEP) {
+        ln_row<T, LPR, R / 2>(nx, x + r * ldx, l, C);
+#pragma unroll
+        for (int i = 0; i < R / 2; i++) keep[i * LPR + l] = nx[i];
+        __builtin_amdgcn_sched_barrier(0);
+        ln_row<T, LPR, R / 2, R / 2>(nx, x + r * ldx, l, C);
+#pragma unroll
+        for (int i = 0; i < R / 2; i++) keep[(R / 2 + i) * LPR + l] = nx[i];
+        asm volatile("" ::: "memory");       // (read back, not held in registers)
+      } else {
+        ln_row<T, LPR, R>(nx, x + r * ldx, l, C);
+      }
       ln_row<T, LPR, R>(nd, dy + r * lddy, l, C);
     }
+    const auto xs = [&](int i) { return KEEP ? keep[i * LPR + l] : nx[KEEP ? 0 : i]; };
     float h[LEAN ? 1 : R][N], g[LEAN ? 1 : R][N];
     float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -198,10 +255,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
         ln_gain<N>(wv[0], wr, (l + i * LPR) * N, C, 1.f);
         __builtin_amdgcn_sched_barrier(0);
       }
+      const LnVec<T> xi = xs(i);
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        const float d = to_f32(nd[i].v[e]);                  // 0 behind the row's end, and so is all it multiplies
-        h[k][e] = (to_f32(nx[i].v[e]) - mean) * rstd;
+        const float d = nd[i].at(e);                         // 0 behind the row's end, and so is all it multiplies
+        h[k][e] = (xi.at(e) - mean) * rstd;
         g[k][e] = d * wv[k][e];
         aw[i][e] += d * h[k][e];
         ab[i][e] += d;
@@ -210,24 +268,24 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void layer_norm_bwd_kernel(
       }
     }
     if (!LEAN && r + gs < rows) {
-      ln_row<T, LPR, R>(nx, x + (r + gs) * ldx, l, C);
+      ln_row<T, LPR, (KEEP ? R / 2 : R)>(nx, x + (r + gs) * ldx, l, C);
       ln_row<T, LPR, R>(nd, dy + (r + gs) * lddy, l, C);
     }
     if (dx) {
       ln_sum<LPR, 2>(s, lds, slot);
       const float c1 = s[0] * inv, c2 = s[1] * inv;
-      if constexpr (LEAN) asm("" : "+s"(wr));
+      if constexpr (LEAN) asm volatile("" : "+s"(wr) : : "memory");
 #pragma unroll
       for (int i = 0; i < R; i++) {
         const int k = LEAN ? 0 : i;
         if constexpr (LEAN) {
-
           ln_gain<N>(wv[0], wr, (l + i * LPR) * N, C, 1.f);
+          const LnVec<T> xi = xs(i);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int e = 0; e < N; e++) {
-            h[0][e] = (to_f32(nx[i].v[e]) - mean) * rstd;
-            g[0][e] = to_f32(nd[i].v[e]) * wv[0][e];
+            h[0][e] = (xi.at(e) - mean) * rstd;
+            g[0][e] = nd[i].at(e) * wv[0][e];
           }
         }
 #pragma unroll
@@ -308,45 +366,45 @@ __global__ __launch_bounds__(1024) void layer_norm_param_kernel(const float* __r
 
 #define LN_MAX_COLS 32768
 
-static inline int ln_groups_per_block(int dtype, int C) {    // rows a workgroup works on at once
-  const int n = dtype == MADIFF_BF16 ? 8 : 4, v = (C + n - 1) / n;
-  if (v > 256) return 1;
+// Lanes a row: 8..64 of one wave, four waves to a workgroup, while 16 elements a lane hold it, else a workgroup of its own.
+static inline int ln_lanes_per_row(int dtype, int C) {
+  const int n = dtype == MADIFF_BF16 ? 8 : 4, v = (C + n - 1) / n, r = v <= 64 ? 1 : 16 / n;
   int lpr = 8;
-  while (lpr < v && lpr < 64) lpr <<= 1;
-  return 256 / lpr;
+  while (lpr * r < v && lpr < 1024) lpr <<= 1;
+  return lpr;
 }
-static inline long ln_blocks(int dtype, long rows, int C, int per_group, int most) {
-  const long gpb = ln_groups_per_block(dtype, C);
+static inline long ln_blocks(int dtype, long rows, int C, int per_group, long lanes) {
+  const int lpr = ln_lanes_per_row(dtype, C), block = lpr > 64 ? lpr : 256;
+  const long gpb = block / lpr, most = lanes / block;
   const long b = (rows + gpb * per_group - 1) / (gpb * per_group);
   return b < 1 ? 1 : (b > most ? most : b);
 }
 
-// calls F<T, LPR, R> for the row width; the widths that R = 1 .. 4 vectors of one wave hold stay in one wave
+// calls F<T, LPR, R> for the row width
 #define LN_DISPATCH(F)                                                   \
   do {                                                                   \
-    constexpr int N = 16 / sizeof(T);                                    \
+    constexpr int N = 16 / sizeof(T), R = 16 / N;                        \
     const int v = (C + N - 1) / N;                                       \
     if (v <= 8) F(8, 1);                                                 \
     else if (v <= 16) F(16, 1);                                          \
     else if (v <= 32) F(32, 1);                                          \
     else if (v <= 64) F(64, 1);                                          \
-    else if (v <= 128) F(64, 2);                                         \
-    else if (v <= 192) F(64, 3);                                         \
-    else if (v <= 256) F(64, 4);                                         \
-    else if (v <= 512) F(256, 2);                                        \
-    else if (v <= 1024) F(256, 4);                                       \
-    else if (v <= 2048) F(1024, 2);                                      \
-    else if (v <= 4096) F(1024, 4);                                      \
-    else if constexpr (N == 4) F(1024, 8);                               \
+    else if (R == 4 && v <= 128) F(64, R / 2);                           \
+    else if (v <= 64 * R) F(64, R);                                      \
+    else if (v <= 128 * R) F(128, R);                                    \
+    else if (v <= 256 * R) F(256, R);                                    \
+    else if (v <= 512 * R) F(512, R);                                    \
+    else if (v <= 1024 * R) F(1024, R);                                  \
+    else F(1024, 2 * R);                                                 \
   } while (0)
 
 template <typename T>
 static int ln_fwd(const T* x, long ldx, T* y, long ldy, const float* w, const float* b, float* mean, float* rstd, long rows,
                   int C, int Cpad, float eps, hipStream_t st) {
   const int dt = sizeof(T) == 2 ? MADIFF_BF16 : MADIFF_F32;
-  const dim3 grid((unsigned)ln_blocks(dt, rows, C, 1, 2048));
+  const dim3 grid((unsigned)ln_blocks(dt, rows, C, 1, 2048 * 256));
 #define LN_F(LPR, R)                                                                                                      \
-  hipLaunchKernelGGL((layer_norm_fwd_kernel<T, LPR, R>), grid, dim3(LPR > 256 ? LPR : 256), 0, st, x, ldx, y, ldy, w, b, \
+  hipLaunchKernelGGL((layer_norm_fwd_kernel<T, LPR, R>), grid, dim3(LPR > 64 ? LPR : 256), 0, st, x, ldx, y, ldy, w, b, \
                      mean, rstd, rows, C, Cpad, eps)
   LN_DISPATCH(LN_F);
 #undef LN_F
@@ -358,7 +416,7 @@ template <typename T>
 static int ln_bwd(const T* x, long ldx, const T* dy, long lddy, const float* w, const float* mean, const float* rstd, T* dx,
                   long lddx, float* part, int groups, long rows, int C, int Cpad, hipStream_t st) {
 #define LN_B(LPR, R)                                                                                                      \
-  hipLaunchKernelGGL((layer_norm_bwd_kernel<T, LPR, R>), dim3(groups), dim3(LPR > 256 ? LPR : 256), 0, st, x, ldx, dy,   \
+  hipLaunchKernelGGL((layer_norm_bwd_kernel<T, LPR, R>), dim3(groups), dim3(LPR > 64 ? LPR : 256), 0, st, x, ldx, dy,   \
                      lddy, w, mean, rstd, dx, lddx, part, rows, C, Cpad)
   LN_DISPATCH(LN_B);
 #undef LN_B
@@ -380,7 +438,7 @@ extern "C" int madiff_layer_norm_fwd(int dtype, const void* x, long ldx, void* y
 
 extern "C" int madiff_layer_norm_groups(int dtype, long rows, int C) {
   if ((dtype != MADIFF_F32 && dtype != MADIFF_BF16) || rows < 0 || C < 1 || C > LN_MAX_COLS) return -1;
-  return (int)ln_blocks(dtype, rows, C, 4, C > 2048 ? 256 : 1024);
+  return (int)ln_blocks(dtype, rows, C, 4, 1024 * 256);
 }
 
 extern "C" int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, long lddy, const float* w,
