@@ -80,8 +80,8 @@ class MuonPlan:
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (p, g, m, ema, shadow) if t is not None)
         if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
             raise ValueError("MuonPlan.step: p, g, m, ema and shadow must not overlap")
-        if state is not None and (state.device != self.device or state.dtype != torch.int32 or state.numel() < 2):
-            raise ValueError(f"MuonPlan.step: state has to be an int32[2] on {self.device}")
+        if state is not None and (state.device != self.device or state.dtype != torch.int32 or state.numel() < 2 or not state.is_contiguous()):
+            raise ValueError(f"MuonPlan.step: state has to be a contiguous int32[2] on {self.device}")
         do_ema = (0 if ema is None else 1) if do_ema is None else int(do_ema)
         if do_ema not in (0, 1, 2) or (do_ema and ema is None):
             raise ValueError(f"MuonPlan.step: do_ema has to be 0, 1 or 2, and 0 without ema, not {do_ema}")

@@ -1677,8 +1677,9 @@ class LayerNorm(torch.autograd.Function):
         # parameter gradients: straight into the flat gradient where a sink is installed, else into fresh tensors
         dw = _sink_view(weight) if want_w else None
         db = _sink_view(bias) if want_b else None
-        live = (want_w or want_b) and all(v is not None and v.is_contiguous()
-                                          for v, want in ((dw, want_w), (db, want_b)) if want)
+        # (one tensor as both: its two sums would meet in one place)
+        live = (want_w or want_b) and weight is not bias and all(v is not None and v.is_contiguous()
+                                                                 for v, want in ((dw, want_w), (db, want_b)) if want)
         dt = lib.BF16 if x2.dtype == torch.bfloat16 else lib.F32
         n, ws = 0, None
         if want_w or want_b:

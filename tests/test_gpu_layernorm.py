@@ -193,6 +193,32 @@ def test_far_mean_and_tiny_and_large_values():
         _close(ops.layer_norm(x, w, b), want["y"], (shift, scale))
 
 
+def test_gradients_straight_into_a_flat_buffer():
+    """As the flat optimizers install it (ops.GradSink): two backward passes add up; one tensor as gain and shift gets both sums."""
+    from madiff_amd import ops
+    rows, C = 77, 96
+    x, dy, w, b = _data(rows, C, torch.float32, seed=8)
+    want = _formula(x, w, b, 1e-5, dy)
+    flat, sink = torch.zeros(3 * C, device=DEV), ops.GradSink()
+    w, b, both = (v.clone().requires_grad_(True) for v in (w, b, w))
+    for k, v in enumerate((w, b, both)):
+        v.grad = flat[k * C:(k + 1) * C]
+        sink.register(v, v.grad)
+    ops.SINK = sink
+    try:
+        for k in (1, 2):
+            ops.layer_norm(x, w, b).backward(dy)
+            for n, v in (("dw", w), ("db", b)):
+                _close(v.grad, (k * want[n][0], k * want[n][1] + 2 * U * want[n][0].abs()), (n, k))
+        same = _formula(x, both, both, 1e-5, dy)
+        ops.layer_norm(x, both, both).backward(dy)
+        _close(flat[2 * C:], (same["dw"][0] + same["db"][0],
+                              same["dw"][1] + same["db"][1] + 2 * U * (same["dw"][0].abs() + same["db"][0].abs())), "both")
+        assert w.grad.data_ptr() == flat.data_ptr()
+    finally:
+        ops.SINK = None
+
+
 def test_empty():
     from madiff_amd import ops
     w, b = torch.ones(9, device=DEV, requires_grad=True), torch.zeros(9, device=DEV, requires_grad=True)
@@ -296,6 +322,7 @@ def test_denoiser_with_layer_norm(prec, monkeypatch):
     import diffuser.models as DM
     from madiff_amd import ops
     monkeypatch.setattr(O, "agent_attention", _normed_attention)
+    monkeypatch.setattr(ops, "_AUTOTUNE", False)         # no variant timed here is left to later tests of the same layer shapes
     kw = dict(dim=16, dim_mults=(1, 4, 8), returns_condition=True, condition_dropout=0.25, env_ts_condition=True)
     ops.set_precision(prec)
     try:

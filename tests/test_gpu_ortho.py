@@ -296,7 +296,8 @@ def test_refusals_on_the_gpu():
                      ((p, g, m), dict(momentum=1.0)), ((p, g, m), dict(steps=0)), ((p.cpu(), g, m), {}),
                      ((p, g, m), dict(shadow=torch.zeros(20, device=DEV))), ((p, g, m), dict(ema=p)),
                      ((p, torch.zeros(40, device=DEV)[::2], m), {}), ((both[:20], both[10:], m), {}), ((both, both[20:], m), {}),
-                     ((p, g, m), dict(do_ema=1, state=torch.zeros(2, device=DEV, dtype=torch.int32))), ((p, g, m), dict(ema=g.clone(), state=torch.zeros(1, device=DEV)))):
+                     ((p, g, m), dict(do_ema=1, state=torch.zeros(2, device=DEV, dtype=torch.int32))), ((p, g, m), dict(ema=g.clone(), state=torch.zeros(1, device=DEV))),
+                     ((p, g, m), dict(ema=g.clone(), state=torch.zeros(4, device=DEV, dtype=torch.int32)[::2]))):
         with pytest.raises(ValueError):
             plan.step(*args, lr=0.1, **kw)
     with pytest.raises(ValueError):
