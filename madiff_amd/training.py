@@ -173,6 +173,10 @@ class Trainer(object):
         # Adam(lr, torch defaults) + EMA over the same parameters as the reference's torch.optim.Adam (training.py:109)
         self.optimizer = OPTIMIZERS[optimizer](diffusion_model, self.ema_model, lr=train_lr, ema_decay=ema_decay,
                                                bucket_mb=bucket_mb, **(optimizer_kwargs or {}))
+        if use_graph and not self.optimizer.graphable:
+            raise NotImplementedError(f"Trainer: use_graph with optimizer={optimizer!r} under data parallelism (its steps are issued "
+                                      "eagerly; leave use_graph at None)")
+        self.use_graph = self.use_graph and self.optimizer.graphable
         self.optimizer.broadcast_parameters(0)
         self.bucket = bucket
         self.n_reference = n_reference

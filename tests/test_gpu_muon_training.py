@@ -17,8 +17,9 @@ A, T, FD, ACT, K, B = 3, 12, 10, 5, 20, 4
 
 
 @pytest.fixture(autouse=True)
-def _clean():
+def _clean(monkeypatch):
     from madiff_amd import ops
+    monkeypatch.setattr(ops, "_AUTOTUNE", False)         # no variant timed here is left to later tests of the same layer shapes
     ops.set_precision("fp32")
     try:
         yield
@@ -111,7 +112,9 @@ def _close(got, ref, opt, steps, what):
     assert float(d.max()) <= 0.3 * opt.lr * steps and float(d.mean()) <= 0.02 * opt.lr, what
 
 
-@pytest.mark.parametrize("dp", [False, True], ids=["single", "dp_1rank_rccl"])
+@pytest.mark.parametrize("dp", [False, pytest.param(True, marks=pytest.mark.skip(
+    reason="aborted once at the end of the capture, by a thread that is not Python's; cause unknown: GraphedTrainStep refuses "
+           "this optimizer under data parallelism"))], ids=["single", "dp_1rank_rccl"])
 def test_replayed_steps_match_eager_ones(dp):
     import torch.distributed as dist
     from madiff_amd import ops
@@ -148,6 +151,37 @@ def test_replayed_steps_match_eager_ones(dp):
             dist.destroy_process_group()
 
 
+def test_data_parallel_steps_match_single_ones():
+    """Eager steps with the gradient's buckets reduced in a 1-rank RCCL group, against steps without one; no capture there."""
+    import torch.distributed as dist
+    from madiff_amd import ops
+    from madiff_amd.trainer import FlatMuonEMA, GraphedTrainStep, train_step
+    dif, results = _build(), []
+    batches = [_batch(s) for s in range(3)]
+    for dp in (False, True):
+        if dp:
+            os.environ["MADIFF_FORCE_DP"] = "1"
+            dist.init_process_group("nccl", init_method="tcp://127.0.0.1:29523", rank=0, world_size=1, device_id=torch.device(DEV))
+        try:
+            m = copy.deepcopy(dif)
+            opt = FlatMuonEMA(m, copy.deepcopy(m), lr=1e-3, ema_decay=0.9, bucket_mb=0.25)
+            for i in range(4):
+                train_step(m, opt, [batches[i % 3], batches[(i + 1) % 3]], do_ema=(2, 0, 1, 1)[i], fold=False)
+            torch.cuda.synchronize()
+            assert opt.dp == dp and opt.graphable != dp and opt.step_count == 4 and (not dp or len(opt.buckets) >= 2)
+            if dp:
+                with pytest.raises(NotImplementedError):
+                    GraphedTrainStep(m, opt, batches[0])
+            results.append((opt.flat_p.clone(), opt.flat_ema.clone()))
+        finally:
+            os.environ.pop("MADIFF_FORCE_DP", None)
+            if dp:
+                dist.destroy_process_group()
+            ops.SINK = None
+    for a, b, what in zip(results[1], results[0], ("weights", "ema")):
+        _close(a, b, opt, 4, what)
+
+
 class _Items(torch.utils.data.Dataset):
     def __init__(self, n):
         b = O.synthetic_batch(n, T, A, FD, ACT, 0, seed=11)
@@ -163,8 +197,8 @@ class _Items(torch.utils.data.Dataset):
         return {k: ({kk: vv[i] for kk, vv in v.items()} if isinstance(v, dict) else v[i]) for k, v in self.b.items()}
 
 
-@pytest.mark.parametrize("prec", ["fp32", "bf16"])
-def test_layer_norm_and_muon_in_the_trainer(prec, tmp_path):
+@pytest.mark.parametrize("prec,env_ts", [("fp32", True), ("fp32", False), ("bf16", True)])
+def test_layer_norm_and_muon_in_the_trainer(prec, env_ts, tmp_path):
     """The operators as a user has them: a denoiser with layer norms, trained by Trainer(optimizer="muon"), eagerly and replayed,
     then sampled from."""
     from diffuser.utils import Trainer
@@ -172,7 +206,7 @@ def test_layer_norm_and_muon_in_the_trainer(prec, tmp_path):
     ops.set_precision(prec)
     runs = []
     for use_graph in (False, True):
-        dif = _build(use_layer_norm=True, env_ts_condition=True)
+        dif = _build(use_layer_norm=True, env_ts_condition=env_ts)
         start = {k: v.detach().clone() for k, v in dif.state_dict().items()}
         tr = Trainer(dif, _Items(B * 2 * 4), None, ema_decay=0.9, train_batch_size=B, train_lr=1e-3, gradient_accumulate_every=2,
                      step_start_ema=3, update_ema_every=2, log_freq=100, sample_freq=0, save_freq=100, eval_freq=0,
@@ -190,8 +224,8 @@ def test_layer_norm_and_muon_in_the_trainer(prec, tmp_path):
         draw = torch.Generator().manual_seed(3)
         x0, z = 0.5 * torch.randn(2, T, A, FD, generator=draw).to(DEV), torch.randn(K, 2, T, A, FD, generator=draw).to(DEV)
         cond = {k: (v.to(DEV) if torch.is_tensor(v) else {kk: vv.to(DEV) for kk, vv in v.items()}) for k, v in b["cond"].items()}
-        plans = [tr.ema_model.conditional_sample(cond, returns=b["returns"].to(DEV), env_ts=b["env_ts"].to(DEV), verbose=False,
-                                                 x_init=x0, step_noise=z, use_graph=g) for g in (True, False)]
+        plans = [tr.ema_model.conditional_sample(cond, returns=b["returns"].to(DEV), verbose=False,
+                                                 env_ts=b["env_ts"].to(DEV) if env_ts else None, x_init=x0, step_noise=z, use_graph=g) for g in (True, False)]
         assert bool(torch.isfinite(plans[0]).all()) and plans[0].shape == (2, T, A, FD)
         assert rel_err(plans[0].cpu(), plans[1].cpu()) < 1e-5       # the same launches, without atomics
         runs.append((opt.flat_p.clone(), opt.flat_ema.clone(), opt))

@@ -170,7 +170,7 @@ def test_two_gloo_ranks_match_one_process():
         assert float((a[k] - v).abs().max()) <= 3 * 485 * 16 * 2.0 ** -24 * 1e-2, k
 
 
-def test_refusals():
+def test_refusals(monkeypatch):
     from diffuser.utils import Trainer
     from madiff_amd.trainer import FlatMuonEMA
     for bad in (dict(momentum=1.0), dict(momentum=-0.1), dict(momentum=float("nan")), dict(weight_decay=-1.0),
@@ -183,6 +183,17 @@ def test_refusals():
         Trainer(_net(), None, None, train_device="cpu", optimizer="adam", optimizer_kwargs=dict(ns_steps=3))
     tr = Trainer(_net(), None, None, train_device="cpu", optimizer="muon", optimizer_kwargs=dict(ns_steps=3, weight_decay=0.1))
     assert isinstance(tr.optimizer, FlatMuonEMA) and tr.optimizer.ns_steps == 3 and tr.optimizer.weight_decay == 0.1
+    monkeypatch.setattr(FlatMuonEMA, "broadcast_parameters", lambda self, src: None)
+    monkeypatch.setenv("MADIFF_FORCE_DP", "1")            # a data-parallel step is not captured
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{28900 + os.getpid() % 400}", rank=0, world_size=1)
+    try:
+        with pytest.raises(NotImplementedError):
+            Trainer(_net(), None, None, train_device="cpu", optimizer="muon", use_graph=True)
+        assert not Trainer(_net(), None, None, train_device="cpu", optimizer="muon").use_graph
+        assert Trainer(_net(), None, None, train_device="cpu", use_graph=True).use_graph
+    finally:
+        dist.destroy_process_group()
     net, (idx, y) = _net(), _data(1)
     opt = FlatMuonEMA(net, None)                          # the HIP step needs the module on a GPU
     ((net(idx[0]) - y[0]) ** 2).mean().backward()
