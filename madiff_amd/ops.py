@@ -1686,8 +1686,7 @@ class LayerNorm(torch.autograd.Function):
             n = 2 * C * lib._lib.madiff_layer_norm_groups(dt, rows, C)
             ws = torch.empty(n, dtype=torch.float32, device=x2.device)
             if not live:
-                fresh = torch.empty(2, C, dtype=torch.float32, device=x2.device)
-                dw, db = fresh[0] if want_w else None, fresh[1] if want_b else None
+                dw, db = torch.empty_like(weight) if want_w else None, torch.empty_like(bias) if want_b else None
         at = stats.data_ptr()
         _timed("layer_norm_bwd_kernel", 0.0, lambda: _launch(x2, lambda st: lib.call(
             "madiff_layer_norm_bwd", dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(), max(dy2.stride(0), width),
