@@ -367,7 +367,7 @@ int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, lo
  * overlap need one each. */
 int madiff_ortho_ws(int batch, int rows, int cols, long* ws_bytes);
 /* 0 when the steps of x <- x (a + b x^2 + c x^4) keep every start in [0, 1] inside what the products' operands hold (|values|
- * < 15), steps is in 1..64 and eps > 0; -1 otherwise, and then madiff_orthogonalize / madiff_muon_step refuse the call. */
+ * < 15), steps is in 1..64 and eps in [1e-30, 1e30); -1 otherwise, and then madiff_orthogonalize / madiff_muon_step refuse the call. */
 int madiff_ortho_check(int steps, float a, float b, float c, float eps);
 int madiff_orthogonalize(int dtype, const void* src, void* dst, int batch, int rows, int cols, int steps, float a, float b,
                          float c, float eps, void* ws, long ws_bytes, madiff_stream_t stream);

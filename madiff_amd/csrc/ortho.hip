@@ -19,6 +19,7 @@
 // blocks, each moved by one asynchronous load instruction of a wave.  A and R are symmetric: only their tiles on and above
 // the diagonal are computed, the others are written as mirror images.
 #include "common.h"
+#include <limits.h>
 #include <math.h>
 #include <string.h>
 #include <algorithm>
@@ -951,7 +952,7 @@ struct NsPlan {                    // start of a plan; matrices and lists follow
 static const long NS_MAGIC = 0x6d7502;
 
 static bool ns_describe(NsMat& m, long at, int rows, int cols, float scale, long& ws) {
-  if (rows < 1 || cols < 1 || at < 0) return false;
+  if (rows < 1 || cols < 1 || at < 0 || at > LONG_MAX - (long)rows * cols) return false;
   m.at = at;
   m.rows = rows;
   m.cols = cols;
@@ -1125,7 +1126,8 @@ static bool ns_fits(int steps, float a, float b, float c, bool pairs) {
 }
 
 extern "C" int madiff_ortho_check(int steps, float a, float b, float c, float eps) {
-  return steps >= 1 && steps <= 64 && eps > 0.f && eps < 1e30f && ns_fits(steps, a, b, c, false) ? 0 : -1;
+  // (eps: 2^11 over it has to be an fp32 number, or a matrix of zeros would come out as NaN)
+  return steps >= 1 && steps <= 64 && eps >= 1e-30f && eps < 1e30f && ns_fits(steps, a, b, c, false) ? 0 : -1;
 }
 
 // Everything about a call on `batch` equal matrices but its pointers

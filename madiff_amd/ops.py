@@ -1752,7 +1752,7 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # the usual quintic: steep at 0, valu
 def _check_newton_schulz(who: str, steps, coefficients, eps):
     a, b, c = (float(v) for v in coefficients)
     if lib._lib.madiff_ortho_check(int(steps), a, b, c, float(eps)) != 0:
-        raise ValueError(f"{who}: steps has to be 1..64, eps positive and {steps} steps of x (a + b x^2 + c x^4) have to keep "
+        raise ValueError(f"{who}: steps has to be 1..64, eps in [1e-30, 1e30) and {steps} steps of x (a + b x^2 + c x^4) have to keep "
                          f"[0, 1] within +-15, not steps={steps}, coefficients={tuple(coefficients)}, eps={eps}")
     return int(steps), a, b, c, float(eps)
 

@@ -133,6 +133,17 @@ def test_zero_nan_and_infinity_stay_in_their_matrix():
     assert bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[4]).all())
 
 
+@pytest.mark.parametrize("shape", [(16, 40), (130, 300)])
+def test_tiny_matrices(shape):
+    """A power of two cancels exactly against the norm, which is summed in 64 bits; zeros stay zeros at the smallest eps."""
+    from madiff_amd import ops
+    x = _grad(shape, 21)
+    want = ops.orthogonalize(x)
+    assert torch.equal(ops.orthogonalize(x * 2.0 ** -70, eps=1e-30), want)
+    assert torch.equal(ops.orthogonalize(x * 2.0 ** 70), want)
+    assert not bool(ops.orthogonalize(torch.zeros_like(x), eps=1e-30).any())
+
+
 def test_strides_empty_streams_and_bits():
     from madiff_amd import ops
     base = _grad((4, 200, 330), 8)

@@ -110,3 +110,15 @@ def test_plan_layout_and_refusals():
     assert L.madiff_muon_step(*args) == -1
     args[18] = p
     assert L.madiff_muon_step(*args) == -1
+
+
+def test_smallest_eps_and_largest_offset():
+    """2^11 / eps has to stay an fp32 number (a zero matrix would be NaN), an offset plus its matrix a 64-bit one."""
+    from madiff_amd import lib
+    L = lib._lib
+    assert L.madiff_ortho_check(5, 3.4445, -4.7750, 2.0315, 1e-30) == 0
+    for eps in (9e-31, 1e-38, 1e-45, 1e30):
+        assert L.madiff_ortho_check(5, 3.4445, -4.7750, 2.0315, eps) == -1, eps
+    need = C.c_long()
+    one = lambda at: L.madiff_muon_plan(1, (C.c_long * 1)(at), (C.c_int * 1)(4), (C.c_int * 1)(5), None, None, 0, C.byref(need))  # noqa: E731
+    assert one(2 ** 63 - 21) == 0 and one(2 ** 63 - 20) == -1 and one(2 ** 63 - 1) == -1
