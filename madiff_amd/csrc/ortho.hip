@@ -59,7 +59,8 @@ struct NsGroup {
   const NsMat* mats;
   NsMat one;
   long ws_stride, at_stride;       // bytes / elements from one matrix of the batch to the next
-  long partials;                   // where the workspace's partial sums begin, in bytes
+  long partials, counters;         // where the workspace's partial sums and their counters begin, in bytes
+  int n_counters;
   unsigned char* ws;
 };
 struct NsTile { int mat, ti, tj; };
@@ -159,6 +160,7 @@ __global__ __launch_bounds__(1024) void ns_norm_kernel(NsGroup grp, NsSource q, 
   const NsMat M = ns_mat(grp, mat);
   const long n = (long)M.rows * M.cols, lo = (long)chunk * NS_CHUNK, hi = min(n, lo + NS_CHUNK);
   constexpr int V = KIND == 1 ? 8 : 4, PASSES = NS_CHUNK / 1024 / V;
+  for (int i = blockIdx.x * 1024 + threadIdx.x; i < grp.n_counters; i += gridDim.x * 1024) ((int*)(grp.ws + grp.counters))[i] = 0;
   double sum = 0.0;
   auto take = [&](float v) { sum += (double)v * (double)v; };
   auto step = [&](float g, float m) {                        // -> the new momentum
@@ -304,7 +306,7 @@ struct NsProduct {
 };
 
 // The workgroups of one launch: tile (ti, tj) of matrix `mat`, slice `part` of `parts` of its reduction.  A tile in several parts leaves
-// fp32 partial sums at `slot` (the first part's slot: part p is at slot + p); ns_join_kernel adds them up.
+// fp32 partial sums at `slot` (the first part's slot: part p is at slot + p); whoever comes last to the tile adds them up.
 struct NsWork { int mat, ti, tj, part, parts, slot, pad0, pad1; };
 struct NsList {
   const NsWork* work;              // null: numbered matrix by matrix, tile by tile, part by part
@@ -649,19 +651,52 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
     step(std::false_type{}, k + 1, f1, f0, 0);
   }
   const int m0 = i0 + wm * (BM / WM), n0 = j0 + wn * (BN / WN);
-  if (t.parts > 1) {                                         // this part's sums, as the lanes hold them
-    float* to = (float*)(grp.ws + grp.partials) + (size_t)(t.slot + t.part) * (BM * BN) + (size_t)wave * (TI * TJ * 1024) + lane * 4;
+  if (t.parts > 1) {
+    // A cut reduction: the parts leave their sums as the lanes hold them, and the workgroup that finds itself the last of its tile
+    // adds them up in part order (the same bits whoever it is) and goes on; nobody waits.  Sums and counter go past the XCDs' own
+    // L2s (agent-scope accesses; the stores have arrived before the count).  Fences instead write back and drop whole L2s: 1300 us
+    // where this takes 734 (2048 x 2048).  The sum as a launch of its own: a Muon step of 75 small matrices 150 us, so 131; 256 x
+    // 2048 144, so 124; 1024 x 5120 421, so 416; only squares lose, 2048 x 2048 had 684 (a tile's sums all go to one workgroup).
+    float* to = (float*)(grp.ws + grp.partials) + (size_t)t.slot * (BM * BN) + (size_t)wave * (TI * TJ * 1024) + lane * 2;
+    int* counter = (int*)(grp.ws + grp.counters) + t.slot;
     ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {
       constexpr int b = decltype(at)::value;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        f32x4 v;
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = acc[b / TJ][b % TJ][4 * g + r];
-        *(f32x4*)(to + b * 1024 + g * 256) = v;
+      for (int g = 0; g < 8; g++) {
+        const float s0 = acc[b / TJ][b % TJ][2 * g], s1 = acc[b / TJ][b % TJ][2 * g + 1];
+        __hip_atomic_store((uint64_t*)(to + (size_t)t.part * (BM * BN) + b * 1024 + g * 128),
+                           __float_as_uint(s0) | (uint64_t)__float_as_uint(s1) << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     });
-    return;
+    __shared__ int before;
+    ns_wait_vm<0>();
+    __syncthreads();
+    if (tid == 0) before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (before != t.parts - 1) return;
+    if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);      // for the next product
+    ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[decltype(at)::value / TJ][decltype(at)::value % TJ][r] = 0.f;
+    });
+#pragma unroll(TI * TJ == 1 ? 4 : 2)
+    for (int p = 0; p < t.parts; p++) {
+      uint64_t v[TI * TJ][8];
+#pragma unroll
+      for (int b = 0; b < TI * TJ; b++)
+#pragma unroll
+        for (int g = 0; g < 8; g++)
+          v[b][g] = __hip_atomic_load((const uint64_t*)(to + (size_t)p * (BM * BN) + b * 1024 + g * 128), __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT);
+      ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {
+        constexpr int b = decltype(at)::value;
+#pragma unroll
+        for (int g = 0; g < 8; g++) {
+          acc[b / TJ][b % TJ][2 * g] += __uint_as_float((uint32_t)v[b][g]);
+          acc[b / TJ][b % TJ][2 * g + 1] += __uint_as_float((uint32_t)(v[b][g] >> 32));
+        }
+      });
+    }
   }
   __syncthreads();                                           // the stages are free from here on
   const NsFinish<KIND, OUT, BX> fin(grp, q, M, (uint32_t*)smem + wave * (32 * 33), lane);
@@ -673,41 +708,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
     if constexpr (t1 < TI * TJ) fin.fetch(then, m0 + t1 / TJ * 32, n0 + t1 % TJ * 32);
     fin.finish(now, acc[t0 / TJ][t0 % TJ], m0 + t0 / TJ * 32, n0 + t0 % TJ * 32);
   });
-}
-
-// Tiles whose reduction was cut: the partial sums in part order, then the same ending.  One wave for one wave's row of blocks.
-template <int KIND, int BM, int BN, int WM, int WN, int OUT>
-__global__ __launch_bounds__(64) void ns_join_kernel(NsGroup grp, NsProduct q, NsList list) {
-  constexpr int NW = WM * WN, TI = BM / WM / 32, TJ = BN / WN / 32, BX = BM > BN ? BM : BN;
-  __shared__ uint32_t turn[32 * 33];
-  const int id = blockIdx.x / (NW * TI), sub = blockIdx.x % (NW * TI), wave = sub / TI, i = sub % TI, lane = threadIdx.x;
-  NsWork t;
-  if (list.work) {
-    t = list.work[id];
-  } else {                                                   // tiles matrix by matrix: their first part
-    t = ns_work<KIND == NS_APPLY, BM, BN>(grp, list, id / list.tiles * list.tiles * list.parts + id % list.tiles);
-  }
-  const NsMat M = ns_mat(grp, t.mat);
-  const float* from = (const float*)(grp.ws + grp.partials) + (size_t)t.slot * (BM * BN) + (size_t)wave * (TI * TJ * 1024) +
-                      i * (TJ * 1024) + lane * 4;
-  const int m0 = t.ti * BM + wave / WN * (BM / WM) + i * 32, n0 = t.tj * BN + wave % WN * (BN / WN);
-  const NsFinish<KIND, OUT, BX> fin(grp, q, M, turn, lane);
-#pragma unroll
-  for (int j = 0; j < TJ; j++) {
-    typename NsFinish<KIND, OUT, BX>::Extra x;
-    fin.fetch(x, m0, n0 + j * 32);
-    f32x16 sum;
-#pragma unroll
-    for (int r = 0; r < 16; r++) sum[r] = 0.f;
-    for (int p = 0; p < t.parts; p++)
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const f32x4 v = *(const f32x4*)(from + (size_t)p * (BM * BN) + j * 1024 + g * 256);
-#pragma unroll
-        for (int r = 0; r < 4; r++) sum[4 * g + r] += v[r];
-      }
-    fin.finish(x, sum, m0, n0 + j * 32);
-  }
 }
 
 // ------------------------------------------------------------------------------------------------ one workgroup a matrix
@@ -795,8 +795,10 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
     const int tq = (lane & 15) >> 2, tp = lane & 3, odd = (lane >> 4) & 1;
     const int o = (k * lkb + 2 * j + odd) * 1024 + (8 * fh + tq) * 64 + (((tp >> 1) ^ (2 * fh) ^ (2 * odd)) << 4) + 8 * (tp & 1);
     const int o2 = (o + 256) ^ 16;
-    const s16x4 h0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + o)), h1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + o2));
-    const s16x4 l0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + (o ^ 32))), l1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + (o2 ^ 32)));
+    const s16x4 h0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + o));
+    const s16x4 h1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + o2));
+    const s16x4 l0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + (o ^ 32)));
+    const s16x4 l1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(X + (o2 ^ 32)));
     h = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7));
     l = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7));
   };
@@ -902,7 +904,9 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
         }
       __syncthreads();
     }
-    each(N1{}, part_of == slices - 1 ? nb : 0, sb, block, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) { store(S, skb, v, row, col); });
+    each(N1{}, part_of == slices - 1 ? nb : 0, sb, block, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
+      store(S, skb, v, row, col);
+    });
     __syncthreads();
     product(K1{}, N1{}, sb * sb, sb, wave, 0, skb);
     // R = b A + c A A, kept in the accumulators' place until every wave has read A
@@ -946,8 +950,8 @@ static inline bool ns_small(const NsMat& m) { return m.sp <= 128 && ns_small_byt
 // ------------------------------------------------------------------------------------------------ host
 struct NsPlan {                    // start of a plan; matrices and lists follow
   long magic, bytes, ws_bytes, need, partials;       // need: elements the flat buffers must have
-  int mats, chunks, areas, shape[3], works[3], joins[3], pairs, pad_;
-  long at_mats, at_chunks, at_areas, at_works[3], at_joins[3];
+  int mats, chunks, areas, shape[3], works[3], counters, pairs, pad_;
+  long at_mats, at_chunks, at_areas, at_works[3];
 };
 static const long NS_MAGIC = 0x6d7502;
 
@@ -980,7 +984,7 @@ static bool ns_describe(NsMat& m, long at, int rows, int cols, float scale, long
 // the most workgroups (5 of 256 x 2048: A A 6.2 us where 128 x 128 takes 11.8), 128 x 128 loads half as much for the same work
 // (28 of 1024 x 1024: R X 189 us where 64 x 64 takes 275).  256 x 256 with one workgroup a CU reaches four fifths of the matrix rate in
 // its loop but loses it again to its ending and to unfilled rounds (200 us there), 128 x 256 likewise: neither is kept.  Parts pay
-// where there are few tiles (1024 x 5120 alone: A = X X^T 82 us whole, 21 + 8 us in six parts).
+// where there are few tiles (1024 x 5120 alone: A = X X^T 82 us whole, 28 us in three parts).
 struct NsShape { int bm, bn; double full, alone, rest, part; };
 static const NsShape ns_shapes[2] = {{64, 64, 0.25, 0.127, 4.0, 3.0}, {128, 128, 0.70, 0.39, 8.0, 5.0}};
 static inline int ns_ksteps(int kind, int sp, int lp) { return (kind == NS_GRAM ? lp : sp) / 16; }
@@ -994,8 +998,9 @@ static inline int ns_parts(int ksteps, int len) {             // parts of about 
 static inline double ns_tile_time(const NsShape& s, int ksteps, int parts, bool alone) {
   return (double)ksteps / parts * (alone ? s.alone : s.full) + (parts > 1 ? s.part : s.rest);
 }
-static inline double ns_join_time(const NsShape& s, double parts) {   // a launch, and the partial sums written and read
-  return parts > 0 ? 4.5 + parts * s.bm * s.bn * 4 / 4.5e6 : 0.0;
+// a tile's last workgroup fetches the sums of all its parts; everything written and read
+static inline double ns_join_time(const NsShape& s, int parts, double all) {
+  return parts > 1 ? 4.0 + parts * s.bm * s.bn * 4 / 50e3 + all * s.bm * s.bn * 4 / 4.5e6 : 0.0;
 }
 static const int NS_SLOTS = 512;                              // two workgroups a CU
 static const int ns_lens[] = {1 << 30, 512, 320, 256, 192, 160, 128, 112, 96, 80, 64, 56, 48, 40, 32, 24, 16, 12, 8};
@@ -1010,7 +1015,7 @@ static double ns_choose(int kind, int batch, int sp, int lp, int& shape, int& pa
       const double tiles = (double)batch * ns_tiles_of(kind, s, sp, lp), n = tiles * p;
       if (n > (double)NS_MAX_GROUPS) continue;             // (one part a tile of 64 x 64 always fits)
       const double rounds = n <= NS_SLOTS ? 1.0 : n / NS_SLOTS + 0.25;
-      const double t = rounds * ns_tile_time(ns_shapes[s], ks, p, n <= 256.0) + ns_join_time(ns_shapes[s], p > 1 ? n : 0.0);
+      const double t = rounds * ns_tile_time(ns_shapes[s], ks, p, n <= 256.0) + ns_join_time(ns_shapes[s], p, n);
       if (best < 0.0 || t < best) { best = t; shape = s; parts = p; }
     }
   return best;
@@ -1023,17 +1028,14 @@ struct NsRun {                     // one call
   NsGroup grp;
   const int *chunks, *areas;       // norm and split passes: (matrix, chunk), (matrix, ti, tj, 0); null: numbered
   int n_chunks, per_chunks, n_areas, per_areas;
-  int shape[3], joins[3];          // joins: tiles in several parts
+  int shape[3];
   bool pairs;                      // two steps in one go are the faster
-  NsList work[3], join[3];
+  NsList work[3];
 };
 
 template <int KIND, int OUT, int BM, int BN, int D>
 static void ns_go(const NsRun& r, const NsProduct& q, hipStream_t st) {
   hipLaunchKernelGGL((ns_product_kernel<KIND, BM, BN, 2, 2, D, OUT>), dim3(r.work[KIND].n), dim3(256), 0, st, r.grp, q, r.work[KIND]);
-  if (r.joins[KIND] > 0)
-    hipLaunchKernelGGL((ns_join_kernel<KIND, BM, BN, 2, 2, OUT>), dim3(r.joins[KIND] * (BM / 16)), dim3(64), 0, st, r.grp, q,
-                       r.join[KIND]);
 }
 template <int KIND, int OUT>
 static void ns_launch(const NsRun& r, const NsProduct& q, hipStream_t st) {
@@ -1155,13 +1157,13 @@ static int ns_uniform(int batch, int rows, int cols, NsRun& r, long& ws_bytes) {
     time[k] = ns_choose(k, batch, m.sp, m.lp, r.shape[k], parts);
     const int tiles = ns_tiles_of(k, r.shape[k], m.sp, m.lp);
     r.work[k] = {nullptr, batch * tiles * parts, tiles, parts};
-    r.join[k] = r.work[k];
-    r.joins[k] = parts > 1 ? batch * tiles : 0;
+    if (parts > 1 && r.work[k].n > r.grp.n_counters) r.grp.n_counters = r.work[k].n;
     const long bytes = parts > 1 ? (long)r.work[k].n * ns_shapes[r.shape[k]].bm * ns_shapes[r.shape[k]].bn * 4 : 0;
     slots = bytes > slots ? bytes : slots;
   }
   r.pairs = ns_pairs(time);
-  ws_bytes = ws * batch + slots;
+  r.grp.counters = ws * batch + slots;
+  ws_bytes = r.grp.counters + ((long)r.grp.n_counters * 4 + 255) / 256 * 256;
   return 0;
 }
 
@@ -1211,6 +1213,7 @@ double ns_plan_time(const std::vector<NsMat>& mats, int kind, int shape, int len
   const NsShape& s = ns_shapes[shape];
   std::vector<std::pair<double, long>> runs;                 // duration, how many
   double n = 0.0, joined = 0.0;
+  int most = 1;
   for (const NsMat& m : mats) n += (double)ns_tiles_of(kind, shape, m.sp, m.lp) * ns_parts(ns_ksteps(kind, m.sp, m.lp), len);
   double total = 0.0;
   for (const NsMat& m : mats) {
@@ -1220,6 +1223,7 @@ double ns_plan_time(const std::vector<NsMat>& mats, int kind, int shape, int len
     runs.push_back({d, c});
     total += d * c;
     if (p > 1) joined += c;
+    most = p > most ? p : most;
   }
   double end = total / NS_SLOTS;
   if (n < 3000.0) {
@@ -1235,13 +1239,12 @@ double ns_plan_time(const std::vector<NsMat>& mats, int kind, int shape, int len
         end = t > end ? t : end;
       }
   }
-  return end + ns_join_time(s, joined);
+  return end + ns_join_time(s, most, joined);
 }
 
 // The order of one list: runs of neighbouring tiles of a matrix go to the XCD with the least work so far, the costly runs first;
 // the XCDs' queues, long reductions first, are then dealt out in turn (workgroup i starts on XCD i % 8), mat = -1 filling the gaps.
-int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out, std::vector<NsWork>& joins, long& partial_bytes,
-             double& best) {
+int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out, int& slots, long& partial_bytes, double& best) {
   int shape = 0, len = 1 << 30;
   best = -1.0;
   for (int s = 0; s < 2; s++)
@@ -1254,7 +1257,7 @@ int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out,
   std::vector<Run> runs;
   std::vector<std::vector<NsWork>> works(mats.size());
   double total = 0.0;
-  int slots = 0;
+  slots = 0;
   auto cost = [&](const NsWork& w) {
     return ns_tile_time(sh, ns_ksteps(kind, mats[w.mat].sp, mats[w.mat].lp), w.parts, false);
   };
@@ -1266,7 +1269,6 @@ int ns_order(const std::vector<NsMat>& mats, int kind, std::vector<NsWork>& out,
         NsWork w = {i, 0, 0, p, parts, parts > 1 ? slots + t * parts : 0, 0, 0};
         ns_tile_at(kind == NS_APPLY, t, m.sp, m.lp, sh.bm, sh.bn, w.ti, w.tj);
         works[i].push_back(w);
-        if (p == 0 && parts > 1) joins.push_back(w);
         total += cost(w);
       }
     if (parts > 1) slots += tiles * parts;
@@ -1316,20 +1318,21 @@ int ns_plan(int n, const long* at, const int* rows, const int* cols, const float
     need = end > need ? end : need;
     if (chunks > NS_MAX_GROUPS || areas > NS_MAX_GROUPS) return -1;
   }
-  std::vector<NsWork> work[3], join[3];
+  std::vector<NsWork> work[3];
   NsPlan h = {};
   double time[3];
   for (int k = 0; k < 3; k++) {
     long bytes = 0;
-    h.shape[k] = ns_order(mats, k, work[k], join[k], bytes, time[k]);
+    int slots = 0;
+    h.shape[k] = ns_order(mats, k, work[k], slots, bytes, time[k]);
     h.works[k] = (int)work[k].size();
-    h.joins[k] = (int)join[k].size();
+    h.counters = slots > h.counters ? slots : h.counters;
     partials = bytes > partials ? bytes : partials;
   }
   h.pairs = ns_pairs(time);
   h.magic = NS_MAGIC;
   h.partials = ws;
-  h.ws_bytes = ws + partials;
+  h.ws_bytes = ws + partials + ((long)h.counters * 4 + 255) / 256 * 256;
   h.need = need;
   h.mats = n;
   h.chunks = (int)chunks;
@@ -1343,10 +1346,7 @@ int ns_plan(int n, const long* at, const int* rows, const int* cols, const float
   h.at_mats = take((long)n * sizeof(NsMat));
   h.at_chunks = take(chunks * 8);
   h.at_areas = take(areas * 16);
-  for (int k = 0; k < 3; k++) {
-    h.at_works[k] = take((long)h.works[k] * sizeof(NsWork));
-    h.at_joins[k] = take((long)h.joins[k] * sizeof(NsWork));
-  }
+  for (int k = 0; k < 3; k++) h.at_works[k] = take((long)h.works[k] * sizeof(NsWork));
   h.bytes = end;
   *need_bytes = h.bytes;
   if (!plan) return 0;
@@ -1361,10 +1361,7 @@ int ns_plan(int n, const long* at, const int* rows, const int* cols, const float
     for (int ti = 0; ti < ns_div_up(mats[i].sp, 64); ti++)
       for (int tj = 0; tj < ns_div_up(mats[i].lp, 64); tj++) { *ar++ = i; *ar++ = ti; *ar++ = tj; *ar++ = 0; }
   }
-  for (int k = 0; k < 3; k++) {
-    memcpy(out + h.at_works[k], work[k].data(), work[k].size() * sizeof(NsWork));
-    if (!join[k].empty()) memcpy(out + h.at_joins[k], join[k].data(), join[k].size() * sizeof(NsWork));
-  }
+  for (int k = 0; k < 3; k++) memcpy(out + h.at_works[k], work[k].data(), work[k].size() * sizeof(NsWork));
   return 0;
 }
 }  // namespace
@@ -1401,6 +1398,8 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   r.grp.mats = (const NsMat*)(dev + h->at_mats);
   r.grp.ws = (unsigned char*)ws;
   r.grp.partials = h->partials;
+  r.grp.n_counters = h->counters;
+  r.grp.counters = h->ws_bytes - ((long)h->counters * 4 + 255) / 256 * 256;
   r.chunks = (const int*)(dev + h->at_chunks);
   r.areas = (const int*)(dev + h->at_areas);
   r.n_chunks = h->chunks;
@@ -1408,9 +1407,7 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   r.per_chunks = r.per_areas = 1;
   for (int k = 0; k < 3; k++) {
     r.shape[k] = h->shape[k];
-    r.joins[k] = h->joins[k];
     r.work[k] = {(const NsWork*)(dev + h->at_works[k]), h->works[k], 1, 1};
-    r.join[k] = {(const NsWork*)(dev + h->at_joins[k]), h->joins[k], 1, 1};
   }
   NsSource q = {};
   q.g = g;

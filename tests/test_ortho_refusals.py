@@ -67,10 +67,10 @@ def test_plan_layout_and_refusals():
     # every chunk, and every tile on and above the diagonal / of the long side, exactly once
     w = blob[:256].view(torch.int64).tolist()
     i32 = lambda lo, n: blob[lo:lo + 4 * n].view(torch.int32).tolist()                                # noqa: E731
-    n_mats, chunks, areas, *rest = i32(40, 14)
-    shapes, works, joins = rest[:3], rest[3:6], rest[6:9]
-    at_mats, at_chunks, at_areas = w[12:15]
-    at_works, at_joins = w[15:18], w[18:21]
+    n_mats, chunks, areas, *rest = i32(40, 12)
+    shapes, works, counters = rest[:3], rest[3:6], rest[6]
+    at_mats, at_chunks, at_areas = w[11:14]
+    at_works = w[14:17]
     up = lambda v, d: -(-v // d)                                                                      # noqa: E731
     sides = [(32 * up(min(r, c), 32), 32 * up(max(r, c), 32)) for _, r, c in mats]
     ck = i32(at_chunks, 2 * chunks)
@@ -91,10 +91,8 @@ def test_plan_layout_and_refusals():
                 assert slot + part not in slots                          # no two parts share a slot
                 slots.add(slot + part)
         assert set(parts) == want and all(len(v) == v[0][1] for v in parts.values())
-        t = i32(at_joins[kind], 8 * joins[kind])
-        joined = [tuple(t[8 * k:8 * k + 3]) for k in range(joins[kind])]
-        assert sorted(joined) == sorted(k for k, v in parts.items() if len(v) > 1)
-        assert (max(slots, default=-1) + 1) * b * b * 4 + w[4] <= ws.value
+        # partial sums, then a counter for every slot
+        assert (max(slots, default=-1) + 1) * b * b * 4 + w[4] + 4 * counters <= ws.value and max(slots, default=-1) < counters + (not slots)
     bad = blob.clone()
     bad[0] ^= 1
     assert L.madiff_muon_plan_ws(bad.data_ptr(), C.byref(ws), C.byref(el)) == -1
