@@ -712,7 +712,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
 
 // ------------------------------------------------------------------------------------------------ one workgroup a matrix
 // A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything: by launches
-// a 16 x 128 matrix took 84 us, next to none of it work; here it takes 26 (64 x 512: 69, 128 x 96: 51; by launches 84 to 92).
+// a 16 x 128 matrix takes 84 us, next to none of it work; here 26 (64 x 512: 69, 128 x 96: 51; by launches 84 to 92).
 // What bounds it is one CU's chain of dependent products, fifteen of them with a barrier or two each.  Sixteen waves deal the
 // 32 x 32 blocks of a product among them (no mirror images: the whole squares are computed); a product that overwrites what it
 // reads keeps its blocks in registers until everybody has read.
@@ -941,9 +941,9 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
   }
 }
 
-// Whatever fits goes through LDS.  Both ways measured, fp32, alone on the chip: one matrix 16 x 128 37 us (by launches 93),
-// 64 x 512 79 (104), 128 x 160 78 (107); a thousand 16 x 128 129 (186), 64 x 512 400 (628), 128 x 160 364 (693); only many tiny
-// ones come out even (4000 of 16 x 16: 398, by launches 380).
+// Whatever fits goes through LDS.  Both ways measured, fp32, a call at a time: one matrix 16 x 128 36 us (by launches 93),
+// 64 x 512 79 (101), 128 x 160 78 (100); a thousand 16 x 128 130 (189), 64 x 512 405 (628), 128 x 160 368 (692); only many tiny
+// ones come out even (4000 of 16 x 16: 399, by launches 382).
 static inline long ns_small_bytes(const NsMat& m) { return 4L * m.sp * m.lp + 4L * m.sp * m.sp; }
 static inline bool ns_small(const NsMat& m) { return m.sp <= 128 && ns_small_bytes(m) <= NS_SMALL_LDS - 128; }
 
