@@ -9,6 +9,7 @@ fails at import) - there is no PyTorch/CPU fallback on this path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import weakref
 from typing import List, Optional, Sequence, Tuple
@@ -1662,7 +1663,7 @@ class LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, C: int, eps: float):
         y, x2, stats = _layer_norm_forward(x, weight, bias, C, eps, True)
         ctx.save_for_backward(x2, weight, bias, stats)
-        ctx.shape, ctx.C = x.shape, C
+        ctx.shape, ctx.C = (None if x.dim() == 2 else x.shape), C
         return y
 
     @staticmethod
@@ -1672,34 +1673,38 @@ class LayerNorm(torch.autograd.Function):
         C = ctx.C
         rows, width = x2.shape
         dy2 = _rows_of(dy, C)
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        want_x, want_w, want_b, _, _ = ctx.needs_input_grad
         dx = torch.empty_like(x2, memory_format=torch.contiguous_format) if want_x else None
-        # parameter gradients: straight into the flat gradient where a sink is installed, else into fresh tensors
-        dw = _sink_view(weight) if want_w else None
-        db = _sink_view(bias) if want_b else None
-        # (one tensor as both: its two sums would meet in one place)
-        live = (want_w or want_b) and weight is not bias and all(v is not None and v.is_contiguous()
-                                                                 for v, want in ((dw, want_w), (db, want_b)) if want)
         dt = lib.BF16 if x2.dtype == torch.bfloat16 else lib.F32
-        n, ws = 0, None
+        dw = db = ws = None
+        n, live = 0, False
         if want_w or want_b:
-            n = 2 * C * lib._lib.madiff_layer_norm_groups(dt, rows, C)
+            n = 2 * C * _layer_norm_groups(dt, rows, C)
             ws = torch.empty(n, dtype=torch.float32, device=x2.device)
+            if SINK is not None and weight is not bias:     # (one tensor as both: its two sums would meet in one place)
+                # straight into the flat gradient
+                dw, db = SINK.get(weight) if want_w else None, SINK.get(bias) if want_b else None
+                live = all(v is not None and v.is_contiguous() for v, want in ((dw, want_w), (db, want_b)) if want)
             if not live:
                 dw, db = torch.empty_like(weight) if want_w else None, torch.empty_like(bias) if want_b else None
         at = stats.data_ptr()
-        _timed("layer_norm_bwd_kernel", 0.0, lambda: _launch(x2, lambda st: lib.call(
-            "madiff_layer_norm_bwd", dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(), max(dy2.stride(0), width),
-            _p(weight), at, at + 4 * rows, _p(dx), width, _p(dw), _p(db), int(live), _p(ws), n, rows, C, width, st)),
-            nbytes=3.0 * rows * C * x2.element_size())
+        args = (dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(), max(dy2.stride(0), width), _p(weight), at,
+                at + 4 * rows, _p(dx), width, _p(dw), _p(db), int(live), _p(ws), n, rows, C, width)
+        _timed("layer_norm_bwd_kernel", 0.0, lambda: _launch(x2, lambda st: lib.call("madiff_layer_norm_bwd", *args, st)),
+               nbytes=3.0 * rows * C * x2.element_size())
         if live:
             for p_, want in ((weight, want_w), (bias, want_b)):
                 if want:
                     SINK.done(p_)
             dw = db = None
-        if dx is not None and len(ctx.shape) != 2:
+        if dx is not None and ctx.shape is not None:
             dx = dx.view(ctx.shape)
         return dx, dw, db, None, None
+
+
+@functools.lru_cache(maxsize=1024)
+def _layer_norm_groups(dt: int, rows: int, C: int) -> int:
+    return lib._lib.madiff_layer_norm_groups(dt, rows, C)
 
 
 def _layer_norm_check(x, weight, bias, C, eps):
