@@ -144,6 +144,30 @@ def test_tiny_matrices(shape):
     assert not bool(ops.orthogonalize(torch.zeros_like(x), eps=1e-30).any())
 
 
+@pytest.mark.parametrize("shape", [(8, 20, 30), (7, 130, 300)])
+def test_batches_in_several_calls(shape, monkeypatch):
+    """A batch too large for one call goes in several: the matrices' results do not depend on where it is cut."""
+    from madiff_amd import ops
+    x = _grad(shape, 31)
+    _check(ops.orthogonalize(x), x)
+    monkeypatch.setattr(ops, "ORTHO_MAX_BATCH", 3)
+    _check(ops.orthogonalize(x), x)
+    monkeypatch.setattr(ops, "ORTHO_WS_BYTES", 1)
+    _check(ops.orthogonalize(x), x)
+
+
+def test_offsets_past_32_bits(monkeypatch):
+    """8400 matrices of 64 x 4096 in one call: 2.2e9 elements, 17.6 GB of workspace."""
+    from madiff_amd import ops
+    monkeypatch.setattr(ops, "ORTHO_WS_BYTES", 1 << 36)
+    x = torch.randn(8400, 64, 4096, device=DEV, dtype=torch.bfloat16, generator=torch.Generator(device=DEV).manual_seed(3))
+    y = ops.orthogonalize(x)
+    pick = [0, 1, 8190, 8191, 8192, 8193, 8399]                # (matrix 8192 begins at element 2^31)
+    _check(y[pick], x[pick])
+    del x, y
+    torch.cuda.empty_cache()
+
+
 def test_strides_empty_streams_and_bits():
     from madiff_amd import ops
     base = _grad((4, 200, 330), 8)
