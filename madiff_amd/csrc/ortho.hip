@@ -234,20 +234,38 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
   __shared__ float tilebuf[64][65];
   __shared__ double part[4];
   const int i0 = t.ti * 64, j0 = t.tj * 64;                  // X rows (short side), columns
-  const int c = threadIdx.x & 63, k0 = threadIdx.x >> 6;
-  float v[16];
+  // four neighbours of a row of the user's a lane, 16 rows a pass; 16 (8) bytes at once from any element-aligned address (one
+  // element a lane and load: 57 us for the 17 M elements of a Muon step's gradient and momentum, so 40, at 5 TB/s)
+  const int c = 4 * (threadIdx.x & 15), k0 = threadIdx.x >> 4;
+  const int col = (M.tall ? i0 : j0) + c, row0 = (M.tall ? j0 : i0) + k0;
+  float v[4][4];
 #pragma unroll
-  for (int u = 0; u < 16; u++) {                             // the piece is on its way while the norm is put together
-    const int r = (M.tall ? j0 : i0) + k0 + 4 * u, col = (M.tall ? i0 : j0) + c;         // in the user's orientation
-    v[u] = 0.f;
-    if (r < M.rows && col < M.cols) {
-      const long e = M.at + (long)r * M.cols + col;
-      if constexpr (KIND == 2) {
-        const float m = q.m[e];
-        v[u] = q.nesterov ? q.rest * (q.g[e] * q.grad_scale) + q.mu * m : m;
+  for (int u = 0; u < 4; u++) {                              // the piece is on its way while the norm is put together
+    const int r = row0 + 16 * u;
+    const long e = M.at + (long)r * M.cols + col;
+    const int n = r < M.rows ? min(4, M.cols - col) : 0;
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (KIND == 1) {
+      const bf16_t* src = (const bf16_t*)q.src;
+      bf16_t h[4];
+      if (n == 4) __builtin_memcpy(h, src + e, 8);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[u][i] = n == 4 ? to_f32(h[i]) : i < n ? to_f32(src[e + i]) : 0.f;
+    } else {
+      const float* src = KIND == 2 ? q.m : (const float*)q.src;
+      if (n == 4) {
+        __builtin_memcpy(v[u], src + e, 16);
+        if constexpr (KIND == 2) __builtin_memcpy(g, q.g + e, 16);
       } else {
-        v[u] = KIND == 1 ? to_f32(((const bf16_t*)q.src)[e]) : ((const float*)q.src)[e];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          v[u][i] = i < n ? src[e + i] : 0.f;
+          if constexpr (KIND == 2) g[i] = i < n ? q.g[e + i] : 0.f;
+        }
       }
+      if constexpr (KIND == 2)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[u][i] = q.nesterov ? q.rest * (g[i] * q.grad_scale) + q.mu * v[u][i] : v[u][i];
     }
   }
   double sum = 0.0;
@@ -260,13 +278,24 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
   const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
   const float inv = (float)((double)NS_SCALE / (norm > (double)q.eps ? norm : (norm <= (double)q.eps ? (double)q.eps : norm)));
 #pragma unroll
-  for (int u = 0; u < 16; u++) {
-    const int k = k0 + 4 * u;
-    if (M.tall) tilebuf[c][k] = v[u] * inv;
-    else tilebuf[k][c] = v[u] * inv;
+  for (int u = 0; u < 4; u++) {
+    const int k = k0 + 16 * u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (M.tall) tilebuf[c + i][k] = v[u][i] * inv;
+      else tilebuf[k][c + i] = v[u][i] * inv;
+    }
     if constexpr (KIND == 2) {
-      const int r = (M.tall ? j0 : i0) + k, col = (M.tall ? i0 : j0) + c;
-      if (q.zero_grad && r < M.rows && col < M.cols) q.g[M.at + (long)r * M.cols + col] = 0.f;
+      const int r = row0 + 16 * u;
+      if (q.zero_grad && r < M.rows) {
+        float* g = q.g + M.at + (long)r * M.cols + col;
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        if (col + 4 <= M.cols) __builtin_memcpy(g, zero, 16);
+        else
+#pragma unroll
+          for (int i = 0; i < 3; i++)
+            if (col + i < M.cols) g[i] = 0.f;
+      }
     }
   }
   __syncthreads();
