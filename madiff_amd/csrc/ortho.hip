@@ -741,30 +741,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
 
 // ------------------------------------------------------------------------------------------------ one workgroup a matrix
 // A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything: by launches
-// a 16 x 128 matrix takes 84 us, next to none of it work; here 26 (64 x 512: 69, 128 x 96: 51; by launches 84 to 92).
-// What bounds it is one CU's chain of dependent products, fifteen of them with a barrier or two each.  Sixteen waves deal the
+// a 16 x 128 matrix takes 84 us, next to none of it work; here 18 (64 x 512: 69, 128 x 96: 51; by launches 84 to 92).
+// What bounds it is one CU's chain of dependent products, fifteen of them with a barrier or two each.  NW waves deal the
 // 32 x 32 blocks of a product among them (no mirror images: the whole squares are computed); a product that overwrites what it
 // reads keeps its blocks in registers until everybody has read.
+// Eight waves up to 64 rows, sixteen (which spill) above: a thousand of 16 x 128 53 us (with sixteen 81, with four 60), of 64 x 512
+// 335 (409), one 128 x 128 71 with sixteen and 81 with eight; a thousand of 128 x 160 the other way round, 389 and 351.
 #define NS_SMALL_LDS 163840
-#define NS_SMALL_BLOCKS 3          // of X a wave: 4 sp lp + 4 sp^2 <= NS_SMALL_LDS leaves at most 39 of them
+#define NS_TINY_LDS 32768
 
-template <int BYTES, bool BF16>
-__global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__ src, void* __restrict__ dst, NsMat one, long stride,
+template <int BYTES, bool BF16, int NW>
+__global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restrict__ src, void* __restrict__ dst, NsMat one, long stride,
                                                        int steps, float a, float b, float c, float eps) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[BYTES == NS_SMALL_LDS ? BYTES - 128 : BYTES];
-  __shared__ double part[16];
+  __shared__ double part[NW];
+  // blocks of X (4 sp lp + 4 sp^2 <= BYTES leaves at most 39, or 7) and of a square a wave
+  constexpr int NX = ((BYTES == NS_SMALL_LDS ? 39 : 7) + NW - 1) / NW, NQ = ((BYTES == NS_SMALL_LDS ? 16 : 4) + NW - 1) / NW;
   const NsMat& M = one;
   const long at0 = (long)blockIdx.x * stride, n = (long)M.rows * M.cols;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 31, fh = lane >> 5, sb = M.sp >> 5, lb = M.lp >> 5, skb = M.sp >> 4, lkb = M.lp >> 4;
   unsigned char *X = smem, *S = smem + 4 * M.sp * M.lp;
-  // X0: eight columns of X an item, at most five a lane, read once and kept while the norm is put together
-  constexpr int ITEMS = (NS_SMALL_LDS / 4 / 8 + 1023) / 1024;
+  // X0: eight columns of X an item, read once and kept while the norm is put together
+  constexpr int ITEMS = (BYTES / 4 / 8 + 64 * NW - 1) / (64 * NW);
   float v0[ITEMS][8];
   double sum = 0.0;
 #pragma unroll
   for (int u = 0; u < ITEMS; u++) {
-    const int item = tid + 1024 * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
+    const int item = tid + 64 * NW * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
     const long e = M.tall ? at0 + (long)col * M.cols + row : at0 + (long)row * M.cols + col;
     const bool in = row < M.s;
     if (!M.tall && in && col + 8 <= M.l) {
@@ -794,12 +798,12 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
   __syncthreads();
   sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < 16; w++) sum += part[w];
+  for (int w = 0; w < NW; w++) sum += part[w];
   const double norm = sqrt(sum);
   const float inv = (float)((double)NS_SCALE / (norm > (double)eps ? norm : (norm <= (double)eps ? (double)eps : norm)));
 #pragma unroll
   for (int u = 0; u < ITEMS; u++) {
-    const int item = tid + 1024 * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
+    const int item = tid + 64 * NW * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
     if (row >= M.sp) continue;
     f16x8 h, l;
 #pragma unroll
@@ -831,15 +835,15 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
     h = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7));
     l = __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  f32x16 acc[NS_SMALL_BLOCKS];
-  // kind 0: X X^T, 1: S S, 2: S X, steps k0 to k1; block number first + 16 u of the result.  The large and the small
+  f32x16 acc[NX > NQ ? NX : NQ];
+  // kind 0: X X^T, 1: S S, 2: S X, steps k0 to k1; block number first + NW u of the result.  The large and the small
   // products go into sums of their own: one chain would be three latencies long a step.
   struct Pair { f16x8 ah, al, bh, bl; };
   auto product = [&](auto kind, auto most, int blocks, int cols, int first, int k0, int k1) __attribute__((always_inline)) {
     constexpr int KIND = decltype(kind)::value, MOST = decltype(most)::value;
     ns_unroll<MOST>([&](auto uu) __attribute__((always_inline)) {
       constexpr int u = decltype(uu)::value;
-      const int id = first + 16 * u;
+      const int id = first + NW * u;
       if (id >= blocks) return;
       const int i = id / cols, j = id - i * cols;
       auto load = [&](Pair& f, int k) __attribute__((always_inline)) {
@@ -871,7 +875,7 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
   auto each = [&](auto most, int blocks, int cols, int first, auto f) __attribute__((always_inline)) {
     ns_unroll<2 * decltype(most)::value>([&](auto at) __attribute__((always_inline)) {
       constexpr int u = decltype(at)::value / 2, p = decltype(at)::value % 2;
-      const int id = first + 16 * u;
+      const int id = first + NW * u;
       if (id >= blocks) return;
       const int i = id / cols, j = id - i * cols;
       float v[8];
@@ -905,14 +909,14 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
   using K0 = std::integral_constant<int, 0>;
   using K1 = std::integral_constant<int, 1>;
   using K2 = std::integral_constant<int, 2>;
-  using N1 = std::integral_constant<int, 1>;                 // 16 blocks of a square at most
-  using NB = std::integral_constant<int, NS_SMALL_BLOCKS>;
-  const int slices = max(1, min(sb == 1 ? 8 : sb == 2 ? 4 : 1, lkb / 4));
+  using NQs = std::integral_constant<int, NQ>;
+  using NXs = std::integral_constant<int, NX>;
+  const int slices = max(1, min(min(8, NW / (sb * sb)), lkb / 4));
   for (int step = 0; step < steps; step++) {
     // A = X X^T has few blocks and a long reduction: `slices` waves share a block, each adding its part to what the one before it
     // left in the block's own place
     const int nb = sb * sb, part_of = wave / nb, block = part_of < slices ? wave - part_of * nb : nb;
-    product(K0{}, N1{}, nb, sb, block, lkb * part_of / slices, lkb * (part_of + 1) / slices);
+    product(K0{}, NQs{}, nb, sb, block, lkb * part_of / slices, lkb * (part_of + 1) / slices);
     for (int t = 0; t + 1 < slices; t++) {
       f32x4* mine = (f32x4*)(S + block * 4096) + lane;
       if (block < nb && part_of == t)
@@ -933,14 +937,14 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
         }
       __syncthreads();
     }
-    each(N1{}, part_of == slices - 1 ? nb : 0, sb, block, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
+    each(NQs{}, part_of == slices - 1 ? nb : 0, sb, block, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
       store(S, skb, v, row, col);
     });
     __syncthreads();
-    product(K1{}, N1{}, sb * sb, sb, wave, 0, skb);
+    product(K1{}, NQs{}, sb * sb, sb, wave, 0, skb);
     // R = b A + c A A, kept in the accumulators' place until every wave has read A
-    float keep[2][8];
-    each(N1{}, sb * sb, sb, wave, [&](float (&v)[8], int row, int col, auto at) __attribute__((always_inline)) {
+    float keep[2 * NQ][8];
+    each(NQs{}, sb * sb, sb, wave, [&](float (&v)[8], int row, int col, auto at) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] *= c;
       add(v, S, skb, row, col, b);
@@ -948,20 +952,20 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
       for (int e = 0; e < 8; e++) keep[decltype(at)::value][e] = v[e];
     });
     __syncthreads();
-    each(N1{}, sb * sb, sb, wave, [&](float (&)[8], int row, int col, auto at) __attribute__((always_inline)) {
+    each(NQs{}, sb * sb, sb, wave, [&](float (&)[8], int row, int col, auto at) __attribute__((always_inline)) {
       store(S, skb, keep[decltype(at)::value], row, col);
     });
     __syncthreads();
-    product(K2{}, NB{}, sb * lb, lb, wave, 0, skb);
+    product(K2{}, NXs{}, sb * lb, lb, wave, 0, skb);
     __syncthreads();                                         // X has been read: a X is added from a block's own place
-    each(NB{}, sb * lb, lb, wave, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
+    each(NXs{}, sb * lb, lb, wave, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
       add(v, X, lkb, row, col, a);
       store(X, lkb, v, row, col);
     });
     __syncthreads();
   }
   // out of the split form (22 bits: a last rounding of 2^-23), along the user's rows
-  for (long e = tid; e < n; e += 1024) {
+  for (long e = tid; e < n; e += 64 * NW) {
     const int r = (int)(e / M.cols), cc = (int)(e - (long)r * M.cols), row = M.tall ? cc : r, col = M.tall ? r : cc;
     const unsigned char* at = X + ns_chunk(row, col & ~7, 0, lkb) + (col & 7) * 2;
     const float v = ((float)*(const _Float16*)at + (float)*(const _Float16*)(smem + ((at - smem) ^ 32))) * (1.f / NS_SCALE);
@@ -970,9 +974,8 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const void* __restrict__
   }
 }
 
-// Whatever fits goes through LDS.  Both ways measured, fp32, a call at a time: one matrix 16 x 128 36 us (by launches 93),
-// 64 x 512 79 (101), 128 x 160 78 (100); a thousand 16 x 128 130 (189), 64 x 512 405 (628), 128 x 160 368 (692); only many tiny
-// ones come out even (4000 of 16 x 16: 399, by launches 382).
+// Whatever fits goes through LDS.  Both ways measured, fp32, a call at a time: one matrix 16 x 128 29 us (by launches 93),
+// 64 x 512 79 (101), 128 x 160 78 (100); a thousand 16 x 128 53 (189), 64 x 512 335 (628), 128 x 160 389 (692).
 static inline long ns_small_bytes(const NsMat& m) { return 4L * m.sp * m.lp + 4L * m.sp * m.sp; }
 static inline bool ns_small(const NsMat& m) { return m.sp <= 128 && ns_small_bytes(m) <= NS_SMALL_LDS - 128; }
 
@@ -1212,12 +1215,14 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
   if (!src || !dst || (need > 0 && (!ws || ws_bytes < need || ((size_t)ws & 255)))) return -1;
   const NsMat& m = r.grp.one;
   if (ns_small(m)) {
-#define NS_GO(BYTES, BF16)                                                                                                        \
-  hipLaunchKernelGGL((ns_small_kernel<BYTES, BF16>), dim3(batch), dim3(1024), 0, stream, src, dst, m, r.grp.at_stride, steps, a, b, c, \
-                     eps)
-    const bool tiny = ns_small_bytes(m) <= 32768;             // several workgroups a CU
-    if (dtype == MADIFF_BF16) { if (tiny) NS_GO(32768, true); else NS_GO(NS_SMALL_LDS, true); }
-    else { if (tiny) NS_GO(32768, false); else NS_GO(NS_SMALL_LDS, false); }
+#define NS_GO(BYTES, BF16, NW)                                                                                                    \
+  hipLaunchKernelGGL((ns_small_kernel<BYTES, BF16, NW>), dim3(batch), dim3(64 * NW), 0, stream, src, dst, m, r.grp.at_stride, steps, \
+                     a, b, c, eps)
+#define NS_ANY(BYTES, NW) do { if (dtype == MADIFF_BF16) NS_GO(BYTES, true, NW); else NS_GO(BYTES, false, NW); } while (0)
+    if (ns_small_bytes(m) <= NS_TINY_LDS) NS_ANY(NS_TINY_LDS, 8);           // several workgroups a CU
+    else if (m.sp <= 64) NS_ANY(NS_SMALL_LDS, 8);
+    else NS_ANY(NS_SMALL_LDS, 16);
+#undef NS_ANY
 #undef NS_GO
     MADIFF_CHECK_LAUNCH();
     return 0;
