@@ -1642,18 +1642,64 @@ def _rows_of(x: torch.Tensor, C: int) -> torch.Tensor:
     return x2
 
 
+def _layer_norm_call(name, t, entry, args, nbytes):
+    if TIMER is None and GRAPH_TIMER is None and not _ABLATE:
+        dev = t.device.index
+        if torch._C._cuda_getDevice() == dev:          # (what _launch does, without a closure: it runs in the autograd thread)
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(dev))
+            if rc != 0:
+                raise RuntimeError(f"{name} failed with status {rc}")
+            return
+    _timed(name, 0.0, lambda: _launch(t, lambda st: lib.call(entry.__name__, *args, st)), nbytes=nbytes)
+
+
 def _layer_norm_forward(x, weight, bias, C, eps, want_stats):
     """-> (y like x, x as rows, [2, rows] mean and rstd); columns behind C (pad columns of the cl format) come back as zeros."""
-    x2 = _rows_of(x, C)
+    x2 = x if x.dim() == 2 and x.is_contiguous() else _rows_of(x, C)
     rows, width = x2.shape
     y = torch.empty_like(x2, memory_format=torch.contiguous_format)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if want_stats else None
-    at = stats.data_ptr() if want_stats else None
-    _timed("layer_norm_fwd_kernel", 0.0, lambda: _launch(x, lambda st: lib.call(
-        "madiff_layer_norm_fwd", lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x2.data_ptr(),
-        max(x2.stride(0), width), y.data_ptr(), width, _p(weight), _p(bias), at, at + 4 * rows if want_stats else None, rows, C,
-        width, eps, st)), nbytes=2.0 * rows * C * x.element_size())
+    stats, at, at2 = None, None, None
+    if want_stats:
+        stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+        at = stats.data_ptr()
+        at2 = at + 4 * rows
+    _layer_norm_call("layer_norm_fwd_kernel", x, lib._lib.madiff_layer_norm_fwd, (
+        lib.BF16 if x.dtype == torch.bfloat16 else lib.F32, x2.data_ptr(), max(x2.stride(0), width), y.data_ptr(), width, _p(weight),
+        _p(bias), at, at2, rows, C, width, eps), 2.0 * rows * C * x.element_size())
     return y if x.dim() == 2 else y.view(x.shape), x2, stats
+
+
+def _layer_norm_backward(ctx, dy):
+    x2, weight, bias, stats = ctx.saved_tensors
+    C, shape = ctx.C, ctx.shape
+    rows, width = x2.shape
+    dy2 = dy if shape is None and dy.is_contiguous() else _rows_of(dy, C)
+    want_x, want_w, want_b, _, _ = ctx.needs_input_grad
+    dx = torch.empty_like(x2, memory_format=torch.contiguous_format) if want_x else None
+    dt = lib.BF16 if x2.dtype == torch.bfloat16 else lib.F32
+    dw = db = ws = None
+    n, live = 0, False
+    if want_w or want_b:
+        n = 2 * C * _layer_norm_groups(dt, rows, C)
+        ws = stats.new_empty(n)
+        if SINK is not None and weight is not bias:         # (one tensor as both: its two sums would meet in one place)
+            # straight into the flat gradient
+            dw, db = SINK.get(weight) if want_w else None, SINK.get(bias) if want_b else None
+            live = all(v is not None and v.is_contiguous() for v, want in ((dw, want_w), (db, want_b)) if want)
+        if not live:
+            dw, db = torch.empty_like(weight) if want_w else None, torch.empty_like(bias) if want_b else None
+    at = stats.data_ptr()
+    _layer_norm_call("layer_norm_bwd_kernel", x2, lib._lib.madiff_layer_norm_bwd, (
+        dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(), max(dy2.stride(0), width), _p(weight), at, at + 4 * rows,
+        _p(dx), width, _p(dw), _p(db), live, _p(ws), n, rows, C, width), 3.0 * rows * C * x2.element_size())
+    if live:
+        for p_, want in ((weight, want_w), (bias, want_b)):
+            if want:
+                SINK.done(p_)
+        dw = db = None
+    if dx is not None and shape is not None:
+        dx = dx.view(shape)
+    return dx, dw, db, None, None
 
 
 class LayerNorm(torch.autograd.Function):
@@ -1667,39 +1713,12 @@ class LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x2, weight, bias, stats = ctx.saved_tensors
-        C = ctx.C
-        rows, width = x2.shape
-        dy2 = _rows_of(dy, C)
-        want_x, want_w, want_b, _, _ = ctx.needs_input_grad
-        dx = torch.empty_like(x2, memory_format=torch.contiguous_format) if want_x else None
-        dt = lib.BF16 if x2.dtype == torch.bfloat16 else lib.F32
-        dw = db = ws = None
-        n, live = 0, False
-        if want_w or want_b:
-            n = 2 * C * _layer_norm_groups(dt, rows, C)
-            ws = torch.empty(n, dtype=torch.float32, device=x2.device)
-            if SINK is not None and weight is not bias:     # (one tensor as both: its two sums would meet in one place)
-                # straight into the flat gradient
-                dw, db = SINK.get(weight) if want_w else None, SINK.get(bias) if want_b else None
-                live = all(v is not None and v.is_contiguous() for v, want in ((dw, want_w), (db, want_b)) if want)
-            if not live:
-                dw, db = torch.empty_like(weight) if want_w else None, torch.empty_like(bias) if want_b else None
-        at = stats.data_ptr()
-        args = (dt, x2.data_ptr(), max(x2.stride(0), width), dy2.data_ptr(), max(dy2.stride(0), width), _p(weight), at,
-                at + 4 * rows, _p(dx), width, _p(dw), _p(db), int(live), _p(ws), n, rows, C, width)
-        _timed("layer_norm_bwd_kernel", 0.0, lambda: _launch(x2, lambda st: lib.call("madiff_layer_norm_bwd", *args, st)),
-               nbytes=3.0 * rows * C * x2.element_size())
-        if live:
-            for p_, want in ((weight, want_w), (bias, want_b)):
-                if want:
-                    SINK.done(p_)
-            dw = db = None
-        if dx is not None and ctx.shape is not None:
-            dx = dx.view(ctx.shape)
-        return dx, dw, db, None, None
+        # create_graph=True: a graph of the gradients that refuses a second derivative (the wrapper costs a plain call 3 us)
+        return (_layer_norm_backward_once if torch.is_grad_enabled() else _layer_norm_backward)(ctx, dy)
+
+
+_layer_norm_backward_once = once_differentiable(_layer_norm_backward)
 
 
 @functools.lru_cache(maxsize=1024)
