@@ -219,6 +219,24 @@ def test_gradients_straight_into_a_flat_buffer():
         ops.SINK = None
 
 
+def test_launches_are_timed_by_name():
+    """Under the per-launch timer the calls go another way in Python: the same results, and a record each."""
+    from madiff_amd import ops
+    x, dy, w, b = _data(33, 200, torch.bfloat16, seed=4)
+    x, w, b = (v.requires_grad_(True) for v in (x, w, b))
+    run = lambda: (lambda y: (y.detach(), *torch.autograd.grad(y, (x, w, b), dy)))(ops.layer_norm(x, w, b))              # noqa: E731
+    plain = run()
+    ops.TIMER = ops.KernelTimer()
+    try:
+        timed = run()
+        torch.cuda.synchronize()
+        names = [r[0] for r in ops.TIMER.records]
+    finally:
+        ops.TIMER = None
+    assert names == ["layer_norm_fwd_kernel", "layer_norm_bwd_kernel"]
+    assert all(torch.equal(p, q) for p, q in zip(plain, timed))
+
+
 def test_empty():
     from madiff_amd import ops
     w, b = torch.ones(9, device=DEV, requires_grad=True), torch.zeros(9, device=DEV, requires_grad=True)
