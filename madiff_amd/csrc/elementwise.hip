@@ -801,7 +801,7 @@ extern "C" int madiff_event_record_external(void* event, hipStream_t stream) {
 // hipStreamWaitEvent by a non-origin capturing stream appends the waiter to the waited stream's list of parallel capture
 // streams, and hip::Stream::EndCapture() recurses over those lists without a visited set: two side streams that have
 // waited on EACH OTHER (in any order, at any distance) make hipStreamEndCapture recurse until the stack overflows
-// (scripts/dbg/capture_topology.cpp topologies 6/7, profiles/r02_capture_topology.txt).  Returns 1 when the streams are
+// (topologies 6 and 7 of profiles/r02_capture_topology.txt).  Returns 1 when the streams are
 // not both capturing the same graph (the caller then uses an ordinary event record + wait, which is also how a stream
 // JOINS a capture).
 extern "C" int madiff_capture_join(hipStream_t waiter, hipStream_t waited) {
