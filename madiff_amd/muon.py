@@ -74,6 +74,7 @@ class MuonPlan:
         with ema_beta (the default where ema is given), 2 copy; state (int32[2] on the GPU): the mode is state[1] instead
         (none without ema).
         zero_grad: clear g as it is read.  Elements outside the plan's matrices are not touched."""
+        ops._refuse_tangents("MuonPlan.step", p, g, m, ema, shadow)
         ptrs = [self._check(k, t) for k, t in (("p", p), ("g", g), ("m", m))]
         pe = None if ema is None else self._check("ema", ema)
         ps = None if shadow is None else self._check("shadow", shadow, torch.bfloat16)

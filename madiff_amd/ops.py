@@ -15,6 +15,7 @@ import weakref
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import lib
@@ -1634,6 +1635,16 @@ def _launch(t: torch.Tensor, fn) -> None:
         return fn(torch._C._cuda_getCurrentRawStream(dev))
 
 
+def _refuse_tangents(who: str, *tensors) -> None:
+    """Forward-mode differentiation is not there: a dual tensor (which has no requires_grad) would lose its tangent without a
+    word.  (Outside forward_ad.dual_level no tensor has one, and this is one comparison.)"""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{who} has no forward-mode derivative: pass a tensor without a tangent "
+                                   "(torch.autograd.forward_ad.unpack_dual(x).primal)")
+
+
 def _rows_of(x: torch.Tensor, C: int) -> torch.Tensor:
     """x as [rows, ...] with unit column stride and rows that do not overlap; a copy where its strides do not allow that."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
@@ -1748,7 +1759,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x (float32 or bfloat16, up to 32768 columns, any
     strides), in x's type; statistics and arithmetic are float32.  weight, bias: float32 [columns] or None.  Differentiable
-    once in all three; the same call gives the same bits."""
+    once in all three, in reverse mode only; the same call gives the same bits."""
+    _refuse_tangents("layer_norm", x, weight, bias)
     C = x.shape[-1] if torch.is_tensor(x) and x.dim() else 0
     eps = float(eps)
     _layer_norm_check(x, weight, bias, C, eps)
@@ -1786,7 +1798,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     """Newton-Schulz orthogonalisation of x [..., rows, cols] (float32 or bfloat16): every matrix, over max(|x|_F, eps), goes
     `steps` times through  X <- a X + (b A + c A A) X,  A = X X^T on its shorter side; its singular values end up near 1.
     Products are float32-accurate whatever x's type.  Returns a new contiguous tensor of x's shape and type.  Not
-    differentiable: an update is orthogonalised outside autograd."""
+    differentiable, in either mode: an update is orthogonalised outside autograd."""
+    _refuse_tangents("orthogonalize", x)
     if not torch.is_tensor(x) or not x.is_cuda:
         raise ValueError("orthogonalize: x has to be a tensor on the GPU")
     if x.dtype not in (torch.float32, torch.bfloat16):
