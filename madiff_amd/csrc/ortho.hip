@@ -5,12 +5,14 @@
 // The three products are matrix-core work; everything else rides in their epilogues.
 //
 // Arithmetic: the iteration multiplies rounding errors by up to a^steps (485 at the usual coefficients), so 8 or 11 bit
-// operands lose the small directions of G.  Every operand is therefore kept as TWO fp16 numbers, x = hi + lo (hi = x rounded
-// to fp16, lo = the rest rounded to fp16: together 22 bits, 2^-23 of the value at worst), and a product is three fp16 matrix
-// instructions, hi hi + hi lo + lo hi, summed in fp32; the missing lo lo is below 2^-22 of the product.  Measured on the CPU
-// the result is as far from the 64-bit one as an fp32 iteration is.  fp16 holds the range because X, A, R and their products
-// are bounded (|X| <= 1.3 or so, |R| <= 5 at the usual coefficients; other coefficients are checked on the host): they
-// are stored times 2^11, which leaves values down to 2^-25 of the largest their full 22 bits.
+// operands lose the small directions of G.  Every operand is therefore kept as TWO fp16 numbers, 2^11 x = hi + 2^-12 lo: hi is
+// 2^11 x rounded to fp16, lo what is left, times 2^12, rounded (together 22 bits, 2^-23 of the value at worst).  A product is three
+// fp16 matrix instructions, hi hi into one fp32 sum, hi lo + lo hi into another that joins it at the end; the missing lo lo is below
+// 2^-22 of the product.  fp16 holds the range because X, A, R and their products are bounded (|X| <= 1.3 or so, |R| <= 5 at the usual
+// coefficients; other coefficients are checked on the host).  Values keep their 22 bits down to 2^-25; what is smaller is held to a
+// step of 2^-47.  (The second sum is for that: with lo in hi's unit the bits went below 2^-13 already and the step was 2^-35.  Of a 200 x
+// 600 matrix whose other half of rows is 1e-6 times the first, small rows came out 2.4e-3 off, now 8e-7, an fp32 iteration's 2.7e-6.
+// It costs 128 x 128 tiles 34 registers and 7 x 1024 x 5120 2 % of its time.)
 //
 // Storage: a matrix [R, K] (both padded with zeros to multiples of 32) is a grid of blocks of 16 rows x 16 columns, 1 KB each, a
 // row's blocks one after the other.  In a block every row has four 16-byte chunks: hi of columns 0-7, hi of 8-15, lo of 0-7, lo of
@@ -38,6 +40,7 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 
 #define NS_PAD 32                  // both axes of a stored matrix
 #define NS_SCALE 2048.f            // stored value = 2^11 x
+#define NS_LOW 4096.f              // lo is stored 2^12 times as large
 #define NS_CHUNK 16384             // elements a workgroup of the norm pass reads
 #define NS_MAX_SHORT 16384
 #define NS_MAX_LONG (1 << 22)
@@ -121,8 +124,9 @@ __device__ __forceinline__ void ns_split(float v, _Float16& hi, _Float16& lo) { 
   // once from its fp32 rounding, and where those two differ lo belonged to the other one (an error of 2^-11, one value in thousands)
   asm("" : "+v"(v));
   hi = (_Float16)v;
-  lo = (_Float16)(v - (float)hi);
+  lo = (_Float16)((v - (float)hi) * NS_LOW);
 }
+__device__ __forceinline__ float ns_join(_Float16 hi, _Float16 lo) { return (float)hi + (float)lo * (1.f / NS_LOW); }
 
 template <int N> __device__ __forceinline__ void ns_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 template <typename F, int... I>
@@ -446,8 +450,8 @@ struct NsFinish {
       for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int r = 0; r < 8; r++) {
-          v[p][r] += q.c1 * ((float)x.h1[p][r] + (float)x.l1[p][r]);
-          if (KIND == NS_SQUARE && e2) v[p][r] += q.c2 * ((float)x.h2[p][r] + (float)x.l2[p][r]);
+          v[p][r] += q.c1 * ns_join(x.h1[p][r], x.l1[p][r]);
+          if (KIND == NS_SQUARE && e2) v[p][r] += q.c2 * ns_join(x.h2[p][r], x.l2[p][r]);
         }
     if constexpr (OUT == NS_OUT_PLANES) {
       // what no tile computes: the mirror images of tiles to the right of their row of the diagonal
@@ -610,13 +614,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
       f.bl[j] = *(const f16x8*)(S + ((boff ^ swap ^ 32) + j * 2048));
     }
   };
-  f32x16 acc[TI][TJ];
+  f32x16 acc[TI][TJ], low[TI][TJ];     // hi hi, and hi lo + lo hi, which are 2^12 times as large
 #pragma unroll
   for (int i = 0; i < TI; i++)
 #pragma unroll
     for (int j = 0; j < TJ; j++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+      for (int r = 0; r < 16; r++) acc[i][j][r] = low[i][j][r] = 0.f;
   // stage k lives in buffer k % D; stages up to k + D - 2 are on their way when step k begins
 #pragma unroll
   for (int d = 0; d < D - 1; d++)
@@ -666,7 +670,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
           if ((2 * e + 1) * TOTAL / (2 * PIECES) == m) issue(k + D - 1, last, e);
         __builtin_amdgcn_sched_barrier(0);
       }
-      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(part == 0 ? c.bl[j] : c.bh[j], part == 1 ? c.al[i] : c.ah[i], acc[i][j], 0, 0, 0);
+      f32x16& sum = part == 2 ? acc[i][j] : low[i][j];
+      sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(part == 0 ? c.bl[j] : c.bh[j], part == 1 ? c.al[i] : c.ah[i], sum, 0, 0, 0);
     }
     buf = next;
   };
@@ -679,6 +684,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
     step(std::false_type{}, k, f0, f1, 1);
     step(std::false_type{}, k + 1, f1, f0, 0);
   }
+  ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {
+    constexpr int b = decltype(at)::value;
+#pragma unroll
+    for (int r = 0; r < 16; r++) acc[b / TJ][b % TJ][r] += low[b / TJ][b % TJ][r] * (1.f / NS_LOW);
+  });
   const int m0 = i0 + wm * (BM / WM), n0 = j0 + wn * (BN / WN);
   if (t.parts > 1) {
     // A cut reduction: the parts leave their sums as the lanes hold them, and the workgroup that finds itself the last of its tile
@@ -868,7 +878,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
         if (k + 1 < k1) multiply(f1);
       }
 #pragma unroll
-      for (int r = 0; r < 16; r++) acc[u][r] += low[r];
+      for (int r = 0; r < 16; r++) acc[u][r] += low[r] * (1.f / NS_LOW);
     });
   };
   // the lane's values of block u, 16-byte chunk by chunk (columns 32 j + 16 p + 8 fh ..): f(v[8], row, column, number)
@@ -904,7 +914,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
   auto add = [&](float (&v)[8], const unsigned char* P, int kb, int row, int col, float f) {
     const f16x8 h = *(const f16x8*)(P + ns_chunk(row, col, 0, kb)), l = *(const f16x8*)(P + ns_chunk(row, col, 1, kb));
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] += f * ((float)h[e] + (float)l[e]);
+    for (int e = 0; e < 8; e++) v[e] += f * ns_join(h[e], l[e]);
   };
   using K0 = std::integral_constant<int, 0>;
   using K1 = std::integral_constant<int, 1>;
@@ -968,7 +978,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
   for (long e = tid; e < n; e += 64 * NW) {
     const int r = (int)(e / M.cols), cc = (int)(e - (long)r * M.cols), row = M.tall ? cc : r, col = M.tall ? r : cc;
     const unsigned char* at = X + ns_chunk(row, col & ~7, 0, lkb) + (col & 7) * 2;
-    const float v = ((float)*(const _Float16*)at + (float)*(const _Float16*)(smem + ((at - smem) ^ 32))) * (1.f / NS_SCALE);
+    const float v = ns_join(*(const _Float16*)at, *(const _Float16*)(smem + ((at - smem) ^ 32))) * (1.f / NS_SCALE);
     if constexpr (BF16) ((bf16_t*)dst)[at0 + e] = (bf16_t)v;
     else ((float*)dst)[at0 + e] = v;
   }

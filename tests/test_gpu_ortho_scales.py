@@ -1,0 +1,79 @@
+"""Newton-Schulz orthogonalisation of matrices whose rows differ by orders of magnitude, row by row against 64 bits.
+
+Tolerance of one row of X (the shorter side's rows): 5 E32 + (LAST + 2^-23) |row|, E32 the row's error of the same iteration in fp32,
+as test_gpu_ortho derives it for the whole matrix, plus what the stored form leaves out whatever a value's size.  An operand is hi + lo,
+two fp16 numbers at 2^11 and 2^23 times the value, so a value below 2^-25 is held to a step of 2^-47, off by 2^-48 at most.  With s rows
+of length l >= s and |X| <= 1.3: X itself contributes sqrt(l) 2^-48 a row, A the same a row of s numbers, A A twice |A| <= 1.7 times that,
+R = b A + c A A so 4.8 + 2.1 x 3.4 + 1 = 13 times, R X as much times 1.3, and the left-out lo lo of a small value (2^-25 of its own unit
+times 2^-11 of the other's) adds no more than the step once more: below (2 + 2 x 13 x 1.3) sqrt(l) 2^-48 < 36 sqrt(l) 2^-48 a step, which the
+steps that follow magnify at most a = 3.4445 times each: 36 (1 + 3.4 + .. + 3.4^4) = 36 x 198 = 7130 and in all
+FLOOR = 7200 sqrt(l) 2^-48."""
+import math
+
+import pytest
+import torch
+
+from conftest import record_measured
+from test_gpu_ortho import LAST, newton_schulz
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _rows(x):
+    return x.double().square().sum(-1).sqrt()
+
+
+def _check(got, x, what, times=1):
+    """got against the orthogonalised x, row by row of the shorter side; `times` the bound."""
+    want = newton_schulz(x.double())
+    f32 = newton_schulz(x.float()).double()
+    if x.shape[-2] > x.shape[-1]:
+        want, f32, got = want.mT, f32.mT, got.mT
+    floor = 7200 * math.sqrt(want.shape[-1]) * 2.0 ** -48
+    size = _rows(want)
+    bound = 5 * _rows(f32 - want) + (LAST + 2.0 ** -23) * size + floor
+    off = _rows(got.double() - want)
+    assert bool((off <= times * bound).all()), (what, float((off / size).max()), float((off / bound).max()))
+    record_measured(float((off / bound).max()), "of_bound")
+
+
+SHAPES = [(16, 128), (64, 512), (128, 160), (200, 600), (600, 200), (333, 1001), (1024, 1500), (2048, 256)]
+
+
+def _graded(rows, cols, kind, seed=3):
+    x = torch.randn(rows, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed))
+    s = min(rows, cols)
+    f = torch.ones(s, device=DEV)
+    if kind == "one row large":
+        f[s // 3] = 1e6
+    elif kind == "graded":
+        f = torch.logspace(-6, 0, s, device=DEV)
+    else:
+        f[s // 2:] = kind
+    return x * f[:, None] if rows <= cols else x * f
+
+
+@pytest.mark.parametrize("kind", [1e-4, 1e-5, 1e-6, "one row large", "graded"])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_small_rows(rows, cols, kind):
+    from madiff_amd import ops
+    x = _graded(rows, cols, kind)
+    _check(ops.orthogonalize(x), x, (rows, cols, kind))
+
+
+@pytest.mark.parametrize("kind", [1e-5, "one row large"])
+def test_small_rows_of_a_muon_update(kind):
+    """p = 0 and no momentum: one step leaves p = -lr scale O(g), its rows as accurate as the orthogonalised matrix's.  Two steps that
+    share one A are 1.3 to 1.8 times as far off, so twice the bound of one; the update rounds twice more (2 x 2^-24 < 2^-23)."""
+    from madiff_amd.muon import MuonPlan
+    mats, at = [], 0
+    for r, c in SHAPES:
+        mats.append((at, r, c))
+        at += r * c
+    g = torch.cat([_graded(r, c, kind).reshape(-1) for _, r, c in mats])
+    p, m = torch.zeros_like(g), torch.zeros_like(g)
+    MuonPlan(mats, DEV).step(p, g, m, lr=0.5, momentum=0.0, nesterov=False)
+    for o, r, c in mats:
+        x = g[o:o + r * c].view(r, c)
+        _check(p[o:o + r * c].view(r, c) / -0.5, x, (r, c, kind), times=2)
