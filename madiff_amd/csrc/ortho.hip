@@ -12,7 +12,7 @@
 // coefficients; other coefficients are checked on the host).  Values keep their 22 bits down to 2^-25; what is smaller is held to a
 // step of 2^-47.  (The second sum is for that: with lo in hi's unit the bits went below 2^-13 already and the step was 2^-35.  Of a 200 x
 // 600 matrix whose other half of rows is 1e-6 times the first, small rows came out 2.4e-3 off, now 8e-7, an fp32 iteration's 2.7e-6.
-// It costs 128 x 128 tiles 34 registers and 7 x 1024 x 5120 2 % of its time.)
+// It costs 128 x 128 tiles 34 registers; 7 x 1024 x 5120 took 1981 us and takes 1999, 5 x 2048 x 256 156 and 161, 16 x 128 18.2 and 18.7.)
 //
 // Storage: a matrix [R, K] (both padded with zeros to multiples of 32) is a grid of blocks of 16 rows x 16 columns, 1 KB each, a
 // row's blocks one after the other.  In a block every row has four 16-byte chunks: hi of columns 0-7, hi of 8-15, lo of 0-7, lo of
@@ -44,6 +44,7 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
 #define NS_CHUNK 16384             // elements a workgroup of the norm pass reads
 #define NS_MAX_SHORT 16384
 #define NS_MAX_LONG (1 << 22)
+#define NS_MAX_STEPS 64
 #define NS_MAX_GROUPS (1L << 21)   // workgroups of a launch: 2^31 work-items of 1024-lane ones
 
 // One matrix.  Offsets into the user's buffers are in elements, into the workspace in bytes.
@@ -53,7 +54,8 @@ struct NsMat {
   int s, l, sp, lp;                // short / long side, padded
   int tall, parts;                 // rows > cols; number of norm partials
   float scale, pad_;
-  long x, sq, norm;                // X (two buffers of 4 sp lp bytes), squares (four of 4 sp sp), partials (doubles)
+  long x, sq, norm;                // X (two buffers of 4 sp lp bytes), squares (four of 4 sp sp), partials (doubles) and
+                                   // behind them e(0) .. e(steps - 1) and a 0, a byte each (ns_shift)
 };
 
 // What every kernel here gets: the matrices, the tiles, the workspace.  Lists come with a plan; without
@@ -99,6 +101,40 @@ __host__ __device__ inline void ns_tile_at(bool whole, int r, int sp, int lp, in
     while (r >= nj - ti * bm / bn) { r -= nj - ti * bm / bn; ti++; }
     tj = ti * bm / bn + r;
   }
+}
+
+// Matrices below eps start as X = G / eps, of any size.  Step k works on Y = 2^e(k) X, e(k) the most that keeps Y and the next step's
+// result within 1 (0 where X is near 1 already, so nothing changes for other matrices):
+//     Y Y^T = 4^e A        R = b A + c A A = b 4^-e (Y Y^T) + c 16^-e (Y Y^T)^2        Y' = 2^(e(k+1) - e(k)) (a Y + R Y)
+// and the last step takes its shift out.  (Without it |G| = 1e-5 eps came out 3e-4 off and 1e-10 eps as zeros; now 1e-7.)
+struct NsShift {
+  float a, b, c, turn, most;       // the polynomial a + b y + c y^2 of y = x^2, where it turns (or -1), the largest |x| on its orbits
+  int cap;                         // the most an e can be for 2^(11 + e) / eps to be an fp32 number
+};
+// -> e for |X| <= u, and u for the next step
+__device__ __forceinline__ int ns_shift(const NsShift& h, double& u) {
+  const double y = u * u;
+  double grow = fmax(fabs((double)h.a), fabs(h.a + y * (h.b + y * h.c)));
+  if (h.turn > 0.f && h.turn < y) grow = fmax(grow, fabs(h.a + 0.5 * h.b * h.turn));
+  int x;
+  frexp(u * fmax(grow, 1.0), &x);
+  u = fmin(u * grow, (double)h.most);
+  return min(max(-x, 0), h.cap);
+}
+// the table e(0) .. e(steps - 1) where it is not 0
+__device__ __forceinline__ void ns_shifts(const NsShift& h, double u, int steps, unsigned char* to) {
+  for (int k = 0; k < steps; k++) {
+    const int e = ns_shift(h, u);
+    if (e == 0 && fabsf(h.a) >= 1.f) break;                  // X never gets smaller: only 0s from here on
+    to[k] = e;
+  }
+}
+// -> the factor that makes 2^(11 + e(0)) X of an element of G, and u = |X| at the start
+__device__ __forceinline__ float ns_start(const NsShift& h, double norm, float eps, double& u) {
+  u = norm > 0.0 && norm < (double)eps ? norm / (double)eps : 1.0;
+  const double over = norm > (double)eps ? norm : (norm <= (double)eps ? (double)eps : norm);      // (NaN stays)
+  double next = u;
+  return (float)ldexp((double)NS_SCALE / over, ns_shift(h, next));
 }
 
 __device__ __forceinline__ NsMat ns_mat(const NsGroup& g, int mat) {
@@ -151,6 +187,8 @@ struct NsSource {
   float mu, rest, grad_scale;      // rest = 1 - mu, formed in 64 bits by the caller
   int nesterov, zero_grad, bf16;
   float eps;
+  int steps;
+  NsShift shift;
 };
 
 // Partial sums of squares in 64 bits (no gradient is too small or too large), one per NS_CHUNK elements.  Muon: the momentum
@@ -279,8 +317,13 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsGroup grp, NsSource q, 
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
   __syncthreads();
-  const double norm = sqrt(part[0] + part[1] + part[2] + part[3]);
-  const float inv = (float)((double)NS_SCALE / (norm > (double)q.eps ? norm : (norm <= (double)q.eps ? (double)q.eps : norm)));
+  double size;
+  const float inv = ns_start(q.shift, sqrt(part[0] + part[1] + part[2] + part[3]), q.eps, size);
+  if (t.ti == 0 && t.tj == 0 && threadIdx.x == 0) {
+    unsigned char* shifts = grp.ws + M.norm + M.parts * 8L;
+    for (int k = 0; k <= q.steps; k++) shifts[k] = 0;
+    ns_shifts(q.shift, size, q.steps, shifts);
+  }
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     const int k = k0 + 16 * u;
@@ -330,6 +373,7 @@ enum { NS_OUT_PLANES = 0, NS_OUT_F32 = 1, NS_OUT_BF16 = 2, NS_OUT_MUON = 3 };
 struct NsProduct {
   int a, b, e2, out;               // square buffers (SQUARE: A, B^T = B, addend or -1, result) / X buffer read and written (APPLY: b, out)
   float ca, c1, c2;                // result = ca A B + c1 B + c2 E2
+  int step, then;                  // APPLY: from step `step`'s shift to step `then`'s; SQUARE: the shift R is formed at, or -1
   void* dst;                       // last APPLY: the user's buffer
   float *p, *ema;                  // Muon
   bf16_t* shadow;
@@ -373,9 +417,10 @@ struct NsFinish {
   const unsigned char *e1, *e2;
   unsigned char* out;
   int lane, rows, cols, kb, do_ema;
-  float ca;
+  float ca, c1;
 
-  __device__ __forceinline__ NsFinish(const NsGroup& grp, const NsProduct& q_, const NsMat& M_, uint32_t* turn_, int lane_)
+  __device__ __forceinline__ NsFinish(const NsGroup& grp, const NsProduct& q_, const NsMat& M_, uint32_t* turn_, int lane_, int e_now,
+                                      int e_then)
       : q(q_), M(M_), turn(turn_), lane(lane_) {
     const size_t sq = (size_t)M.sp * M.sp * 4, xs = (size_t)M.sp * M.lp * 4;
     rows = M.sp;
@@ -387,6 +432,15 @@ struct NsFinish {
     do_ema = 0;
     if constexpr (OUT == NS_OUT_MUON) do_ema = q.state ? q.state[1] : q.do_ema;
     ca = q.ca * (1.f / NS_SCALE);                            // sums are in units of the scale squared
+    c1 = q.c1;
+    if constexpr (KIND == NS_APPLY) {
+      const float f = ldexpf(1.f, e_then - e_now);
+      ca *= f;
+      c1 *= f;
+    } else if (e_now) {
+      ca = ldexpf(ca, -4 * e_now);
+      c1 = ldexpf(c1, -2 * e_now);
+    }
   }
   // The user's side of the block at (m0, n0): 32 rows of 32 columns; lane & 7 picks four columns, pass k the rows 8 k + lane / 8.
   __device__ __forceinline__ long user(int m0, int n0, int k, int& row, int& col) const {
@@ -450,7 +504,7 @@ struct NsFinish {
       for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int r = 0; r < 8; r++) {
-          v[p][r] += q.c1 * ns_join(x.h1[p][r], x.l1[p][r]);
+          v[p][r] += c1 * ns_join(x.h1[p][r], x.l1[p][r]);
           if (KIND == NS_SQUARE && e2) v[p][r] += q.c2 * ns_join(x.h2[p][r], x.l2[p][r]);
         }
     if constexpr (OUT == NS_OUT_PLANES) {
@@ -558,6 +612,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
   const int kblocks = (KIND == NS_GRAM ? M.lp : M.sp) >> 4;  // a multiple of 2
   const int kfirst = kblocks / 2 * t.part / t.parts * 2, nsteps = kblocks / 2 * (t.part + 1) / t.parts * 2 - kfirst;
   const int i0 = t.ti * BM, j0 = t.tj * BN;
+  const unsigned char* shifts = grp.ws + M.norm + M.parts * 8L;
+  const int e_now = KIND == NS_APPLY || (KIND == NS_SQUARE && q.step >= 0) ? shifts[q.step] : 0, e_then = KIND == NS_APPLY ? shifts[q.then] : 0;
   // this wave's blocks of a stage; blocks of a tile that hangs over the matrix's end repeat its last one
   const unsigned char* src[PIECES];
   size_t hop[PIECES];
@@ -738,7 +794,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
     }
   }
   __syncthreads();                                           // the stages are free from here on
-  const NsFinish<KIND, OUT, BX> fin(grp, q, M, (uint32_t*)smem + wave * (32 * 33), lane);
+  const NsFinish<KIND, OUT, BX> fin(grp, q, M, (uint32_t*)smem + wave * (32 * 33), lane, e_now, e_then);
   typename NsFinish<KIND, OUT, BX>::Extra x0, x1;
   fin.fetch(x0, m0, n0);
   ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {      // (acc lives in registers: its indices are constants)
@@ -762,7 +818,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
 
 template <int BYTES, bool BF16, int NW>
 __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restrict__ src, void* __restrict__ dst, NsMat one, long stride,
-                                                       int steps, float a, float b, float c, float eps) {
+                                                       int steps, float a, float b, float c, float eps, NsShift shift) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[BYTES == NS_SMALL_LDS ? BYTES - 128 : BYTES];
   __shared__ double part[NW];
   // blocks of X (4 sp lp + 4 sp^2 <= BYTES leaves at most 39, or 7) and of a square a wave
@@ -809,8 +865,8 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
   sum = 0.0;
 #pragma unroll
   for (int w = 0; w < NW; w++) sum += part[w];
-  const double norm = sqrt(sum);
-  const float inv = (float)((double)NS_SCALE / (norm > (double)eps ? norm : (norm <= (double)eps ? (double)eps : norm)));
+  double size;
+  const float inv = ns_start(shift, sqrt(sum), eps, size);
 #pragma unroll
   for (int u = 0; u < ITEMS; u++) {
     const int item = tid + 64 * NW * u, row = item / (M.lp / 8), col = (item - row * (M.lp / 8)) * 8;
@@ -827,6 +883,13 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
     *(f16x8*)(X + ns_chunk(row, col, 1, lkb)) = l;
   }
   __syncthreads();
+  // e(0) .. e(63) in the sums' place, read behind the barrier of the first product
+  static_assert(sizeof part >= NS_MAX_STEPS, "a byte each");
+  unsigned char* const shifts = (unsigned char*)part;
+  if (wave == 0) {
+    shifts[lane] = 0;
+    if (lane == 0) ns_shifts(shift, size, steps, shifts);
+  }
   // hi and lo of the rows 32 i .. + 31, columns 16 k .. + 15 of a matrix, as an operand
   auto rows_of = [&](const unsigned char* P, int kb, int i, int k, f16x8& h, f16x8& l) {
     const unsigned char* p = P + ((2 * i + (fr >> 4)) * kb + k) * 1024 + (fr & 15) * 64 + ((fh ^ ((fr >> 2) & 3) ^ ((k & 1) << 1)) << 4);
@@ -953,11 +1016,12 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
     __syncthreads();
     product(K1{}, NQs{}, sb * sb, sb, wave, 0, skb);
     // R = b A + c A A, kept in the accumulators' place until every wave has read A
+    const float bs = ldexpf(b, -2 * shifts[step]), cs = ldexpf(c, -4 * shifts[step]);
     float keep[2 * NQ][8];
     each(NQs{}, sb * sb, sb, wave, [&](float (&v)[8], int row, int col, auto at) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] *= c;
-      add(v, S, skb, row, col, b);
+      for (int e = 0; e < 8; e++) v[e] *= cs;
+      add(v, S, skb, row, col, bs);
 #pragma unroll
       for (int e = 0; e < 8; e++) keep[decltype(at)::value][e] = v[e];
     });
@@ -968,17 +1032,21 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
     __syncthreads();
     product(K2{}, NXs{}, sb * lb, lb, wave, 0, skb);
     __syncthreads();                                         // X has been read: a X is added from a block's own place
+    const float f = ldexpf(1.f, step + 1 < steps ? shifts[step + 1] - shifts[step] : 0), as = a * f;
     each(NXs{}, sb * lb, lb, wave, [&](float (&v)[8], int row, int col, auto) __attribute__((always_inline)) {
-      add(v, X, lkb, row, col, a);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] *= f;
+      add(v, X, lkb, row, col, as);
       store(X, lkb, v, row, col);
     });
     __syncthreads();
   }
+  const float unit = ldexpf(1.f / NS_SCALE, -shifts[steps - 1]);
   // out of the split form (22 bits: a last rounding of 2^-23), along the user's rows
   for (long e = tid; e < n; e += 64 * NW) {
     const int r = (int)(e / M.cols), cc = (int)(e - (long)r * M.cols), row = M.tall ? cc : r, col = M.tall ? r : cc;
     const unsigned char* at = X + ns_chunk(row, col & ~7, 0, lkb) + (col & 7) * 2;
-    const float v = ns_join(*(const _Float16*)at, *(const _Float16*)(smem + ((at - smem) ^ 32))) * (1.f / NS_SCALE);
+    const float v = ns_join(*(const _Float16*)at, *(const _Float16*)(smem + ((at - smem) ^ 32))) * unit;
     if constexpr (BF16) ((bf16_t*)dst)[at0 + e] = (bf16_t)v;
     else ((float*)dst)[at0 + e] = v;
   }
@@ -1017,7 +1085,7 @@ static bool ns_describe(NsMat& m, long at, int rows, int cols, float scale, long
   m.sq = ws;
   ws += 4L * m.sp * m.sp * 4;
   m.norm = ws;
-  ws += (parts * 8 + 255) / 256 * 256;
+  ws += (parts * 8 + NS_MAX_STEPS + 1 + 255) / 256 * 256;
   return true;
 }
 
@@ -1099,8 +1167,9 @@ static void ns_launch_source(const NsRun& r, const NsSource& q, hipStream_t st) 
 static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int out, const NsProduct& last, bool pairs,
                       hipStream_t st) {
   enum { G = 0, R = 1, T = 2, R2 = 3 };
-  auto square = [&](int x, int y, float ca, float c1, int e2, float c2, int to) {        // to = ca x y + c1 y + c2 e2
+  auto square = [&](int x, int y, float ca, float c1, int e2, float c2, int to, int shift = -1) {   // to = ca x y + c1 y + c2 e2
     NsProduct q = {};
+    q.step = shift;
     q.a = x;
     q.b = y;
     q.ca = ca;
@@ -1118,15 +1187,18 @@ static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int 
     q.out = G;
     q.ca = 1.f;
     ns_launch<NS_GRAM, NS_OUT_PLANES>(r, q, st);
-    square(G, G, c, b, -1, 0.f, R);
+    square(G, G, c, b, -1, 0.f, R, k);
     if (two) {
       square(R, G, 1.f, a, -1, 0.f, T);
       square(R, T, 1.f, a, -1, 0.f, G);
-      square(G, G, c, b, -1, 0.f, R2);
+      square(G, G, c, b, -1, 0.f, R2, k);
       square(R2, R, 1.f, a, R2, a, T);
     }
+    const int from = k;
     k += two ? 2 : 1;
     q = k >= steps ? last : NsProduct{};
+    q.step = from;
+    q.then = k;
     q.a = two ? T : R;
     q.b = x;
     q.out = x ^ 1;
@@ -1143,8 +1215,9 @@ static int ns_iterate(const NsRun& r, int steps, float a, float b, float c, int 
 }
 
 // The polynomial's orbit from every start in [0, 1]: the largest |x|, |A| and |R| on it, and what pairs of steps store besides,
-// have to stay in the stored range.
-static bool ns_bounded(int steps, float a, float b, float c, bool pairs) {
+// have to stay in the stored range.  `most`: the largest |x|.
+static bool ns_bounded(int steps, float a, float b, float c, bool pairs, double& most) {
+  most = 1.0;
   const double top = 65504.0 / NS_SCALE / 2;
   auto in = [&](double v) { return v < top && v > -top; };
   for (int i = 0; i <= 4096; i++) {
@@ -1152,6 +1225,7 @@ static bool ns_bounded(int steps, float a, float b, float c, bool pairs) {
     for (int k = 0; k < steps; k++) {
       const double g = x * x, q = b * g + c * g * g;
       x = x * (a + q);
+      most = fmax(most, fabs(x));
       if (!(in(x) && in(g) && in(q))) return false;
       if (pairs && !(in((a + q) * g) && (k % 2 == 0 || in((a + q) * (a + before) - (double)a * a)))) return false;
       before = q;
@@ -1161,17 +1235,24 @@ static bool ns_bounded(int steps, float a, float b, float c, bool pairs) {
 }
 
 // the same, remembered per thread for the last polynomial: walking the orbits takes longer than a small call
-static bool ns_fits(int steps, float a, float b, float c, bool pairs) {
-  struct Last { int steps; float a, b, c; bool fits; };
-  static thread_local Last last[2] = {{-1, 0.f, 0.f, 0.f, false}, {-1, 0.f, 0.f, 0.f, false}};
-  Last& l = last[pairs];
-  if (l.steps != steps || l.a != a || l.b != b || l.c != c) l = {steps, a, b, c, ns_bounded(steps, a, b, c, pairs)};
-  return l.fits;
+struct NsOrbit { int steps; float a, b, c; bool fits; double most; };
+static const NsOrbit& ns_orbit(int steps, float a, float b, float c, bool pairs) {
+  static thread_local NsOrbit last[2] = {{-1, 0.f, 0.f, 0.f, false, 0.0}, {-1, 0.f, 0.f, 0.f, false, 0.0}};
+  NsOrbit& l = last[pairs];
+  if (l.steps != steps || l.a != a || l.b != b || l.c != c) {
+    l = {steps, a, b, c, false, 0.0};
+    l.fits = ns_bounded(steps, a, b, c, pairs, l.most);
+  }
+  return l;
+}
+static bool ns_fits(int steps, float a, float b, float c, bool pairs) { return ns_orbit(steps, a, b, c, pairs).fits; }
+static NsShift ns_shift_of(int steps, float a, float b, float c, float eps) {
+  return {a, b, c, c != 0.f ? -b / (2.f * c) : -1.f, (float)ns_orbit(steps, a, b, c, false).most * 1.01f, 115 + ilogbf(eps)};
 }
 
 extern "C" int madiff_ortho_check(int steps, float a, float b, float c, float eps) {
   // (eps: 2^11 over it has to be an fp32 number, or a matrix of zeros would come out as NaN)
-  return steps >= 1 && steps <= 64 && eps >= 1e-30f && eps < 1e30f && ns_fits(steps, a, b, c, false) ? 0 : -1;
+  return steps >= 1 && steps <= NS_MAX_STEPS && eps >= 1e-30f && eps < 1e30f && ns_fits(steps, a, b, c, false) ? 0 : -1;
 }
 
 // Everything about a call on `batch` equal matrices but its pointers
@@ -1224,10 +1305,11 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
   if (batch == 0) return 0;
   if (!src || !dst || (need > 0 && (!ws || ws_bytes < need || ((size_t)ws & 255)))) return -1;
   const NsMat& m = r.grp.one;
+  const NsShift shift = ns_shift_of(steps, a, b, c, eps);
   if (ns_small(m)) {
 #define NS_GO(BYTES, BF16, NW)                                                                                                    \
   hipLaunchKernelGGL((ns_small_kernel<BYTES, BF16, NW>), dim3(batch), dim3(64 * NW), 0, stream, src, dst, m, r.grp.at_stride, steps, \
-                     a, b, c, eps)
+                     a, b, c, eps, shift)
 #define NS_ANY(BYTES, NW) do { if (dtype == MADIFF_BF16) NS_GO(BYTES, true, NW); else NS_GO(BYTES, false, NW); } while (0)
     if (ns_small_bytes(m) <= NS_TINY_LDS) NS_ANY(NS_TINY_LDS, 8);           // several workgroups a CU
     else if (m.sp <= 64) NS_ANY(NS_SMALL_LDS, 8);
@@ -1241,6 +1323,8 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
   NsSource q = {};
   q.src = src;
   q.eps = eps;
+  q.steps = steps;
+  q.shift = shift;
   if (dtype == MADIFF_BF16) ns_launch_source<1>(r, q, stream);
   else ns_launch_source<0>(r, q, stream);
   MADIFF_CHECK_LAUNCH();
@@ -1462,6 +1546,8 @@ extern "C" int madiff_muon_step(const void* plan, const void* plan_device, float
   q.nesterov = nesterov;
   q.zero_grad = zero_grad;
   q.eps = eps;
+  q.steps = steps;
+  q.shift = ns_shift_of(steps, a, b, c, eps);
   ns_launch_source<2>(r, q, stream);
   MADIFF_CHECK_LAUNCH();
   NsProduct last = {};

@@ -77,3 +77,68 @@ def test_small_rows_of_a_muon_update(kind):
     for o, r, c in mats:
         x = g[o:o + r * c].view(r, c)
         _check(p[o:o + r * c].view(r, c) / -0.5, x, (r, c, kind), times=2)
+
+
+# Matrices below eps start as G / eps, as small as that may be.  The bound is that of one at eps or above, relative to the result's
+# 2-norm: a power of two that keeps the stored values in range changes nothing else, and the growth from there is a per step as ever.
+STARTS = [(steps, coef, eps, part) for steps, coef, eps, parts in (
+    (5, (3.4445, -4.7750, 2.0315), 1e-7, (0.7, 1e-2, 1e-4, 1e-6, 1e-9, 1e-13, 1e-20)), (1, (3.4445, -4.7750, 2.0315), 1e-7, (1e-8,)),
+    (24, (3.4445, -4.7750, 2.0315), 1e-7, (1e-6, 1e-10)), (6, (3.4445, -4.7750, 2.0315), 1e3, (1e-12,)), (4, (1.5, -0.5, 0.0), 1e-12, (1e-5,)),
+    (40, (0.5, 0.25, 0.0), 1e-7, (1e4, 1e-3))) for part in parts]
+
+
+def _start(rows, cols, norm, seed=5):
+    x = torch.randn(rows, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed), dtype=torch.float64)
+    return (x * (norm / float(x.norm()))).float()
+
+
+@pytest.mark.parametrize("steps,coef,eps,part", STARTS)
+def test_matrices_below_eps(steps, coef, eps, part):
+    from madiff_amd import ops
+    for rows, cols in ((16, 128), (130, 40), (300, 500), (128, 160)):
+        x = _start(rows, cols, part * eps)
+        want, f32 = newton_schulz(x.double(), steps, coef, eps), newton_schulz(x, steps, coef, eps).double()
+        got = ops.orthogonalize(x, steps=steps, coefficients=coef, eps=eps).double()
+        bound = 5 * float((f32 - want).norm()) + (LAST + 2.0 ** -23) * float(want.norm())
+        off = float((got - want).norm())
+        assert off <= bound, (rows, cols, off / float(want.norm()), bound / float(want.norm()))
+        record_measured(off / bound, "of_bound")
+        b16 = ops.orthogonalize(x.bfloat16(), steps=steps, coefficients=coef, eps=eps).double()       # two steps in one where they pay
+        want = newton_schulz(x.bfloat16().double(), steps, coef, eps)
+        assert float((b16 - want).norm()) <= 2 * bound + 2.0 ** -8 * float(want.norm()), (rows, cols)
+
+
+def test_matrices_of_all_sizes_together():
+    """One call, one plan: what a matrix's own norm needs is not another's."""
+    from madiff_amd import ops
+    from madiff_amd.muon import MuonPlan
+    parts = [1e6, 1e-3, 1.5, 1e-9, 0.0, 1e-16]
+    for rows, cols in ((200, 300), (24, 50)):
+        x = torch.stack([_start(rows, cols, q * 1e-7, seed=k) if q else torch.zeros(rows, cols, device=DEV) for k, q in enumerate(parts)])
+        got = ops.orthogonalize(x).double()
+        mats = [(k * rows * cols, rows, cols) for k in range(len(parts))]
+        p, m, g = torch.zeros(x.numel(), device=DEV), torch.zeros(x.numel(), device=DEV), x.reshape(-1).clone()
+        MuonPlan(mats, DEV).step(p, g, m, lr=0.5, momentum=0.0, nesterov=False)
+        p = p.view_as(x).double() / -0.5
+        for k, q in enumerate(parts):
+            want, f32 = newton_schulz(x[k].double()), newton_schulz(x[k]).double()
+            bound = 5 * float((f32 - want).norm()) + (LAST + 2.0 ** -23) * float(want.norm())
+            assert float((got[k] - want).norm()) <= bound, (rows, q, float((got[k] - want).norm() / want.norm()))
+            assert float((p[k] - want).norm()) <= 2 * bound, (rows, q, float((p[k] - want).norm() / want.norm()))
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 512), (200, 600), (600, 200)])
+def test_small_columns(rows, cols):
+    """Columns of X (the longer side) keep their bits as rows do: sqrt(s) numbers of a column instead of sqrt(l) of a row."""
+    from madiff_amd import ops
+    x = torch.randn(rows, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(8))
+    l = max(rows, cols)
+    f = torch.ones(l, device=DEV)
+    f[l // 2:] = 1e-6
+    x = x * f if rows < cols else x * f[:, None]
+    want, f32, got = newton_schulz(x.double()), newton_schulz(x).double(), ops.orthogonalize(x).double()
+    if rows < cols:
+        want, f32, got = want.mT, f32.mT, got.mT
+    bound = 5 * _rows(f32 - want) + (LAST + 2.0 ** -23) * _rows(want) + 7200 * math.sqrt(min(rows, cols)) * 2.0 ** -48
+    off = _rows(got - want)
+    assert bool((off <= bound).all()), float((off / bound).max())
