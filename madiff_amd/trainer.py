@@ -561,7 +561,7 @@ class FlatMuonEMA(FlatAdamEMA):
                 u, w = u.transpose(0, 1), w.transpose(0, 1)
             x = u.reshape(rows, cols)
             x = x.T if rows > cols else x
-            x = x / (x.norm() + 1e-7)
+            x = x / x.norm().clamp_min(1e-7)
             for _ in range(self.ns_steps):
                 r = x @ x.T
                 x = a * x + (b * r + c * (r @ r)) @ x

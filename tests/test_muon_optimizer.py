@@ -199,3 +199,30 @@ def test_refusals(monkeypatch):
     ((net(idx[0]) - y[0]) ** 2).mean().backward()
     with pytest.raises(RuntimeError):
         opt.step()
+
+
+def test_gradients_below_eps():
+    """|U| around and far below eps = 1e-7: X starts as U / max(|U|, eps), so the update of a matrix shrinks with its gradient and is
+    that of a unit matrix from eps on.  The bound is that of the header, relative to the update."""
+    from madiff_amd.trainer import FlatMuonEMA
+    a, b, c = NS
+    lr = 1e-2
+    for size in (1e-5, 3e-7, 0.9e-7, 1e-9, 1e-13):
+        net, (idx, y) = _net(), _data(1)
+        opt = FlatMuonEMA(net, None, lr=lr, momentum=0.0, nesterov=False, use_hip_kernel=False)
+        ((net(idx[0]) - y[0]) ** 2).mean().backward()
+        opt.step()
+        opt.zero_grad()
+        g = torch.randn(8, 18, generator=torch.Generator().manual_seed(4), dtype=torch.float64)
+        g = (g * (size / g.norm())).float()
+        opt.flat_m.zero_()
+        net.conv.weight.grad.copy_(g.view(8, 6, 3))
+        opt.flat_p.zero_()                                # (so that the update does not drown in the weights)
+        opt.step()
+        x = g.double() / max(float(g.double().norm()), 1e-7)
+        for _ in range(5):
+            r = x @ x.T
+            x = a * x + (b * r + c * r @ r) @ x
+        want = -lr * 0.2 * math.sqrt(18) * x
+        got = net.conv.weight.detach().double().reshape(8, 18)
+        assert float((got - want).norm()) <= 0.007 * float(want.norm()), size
