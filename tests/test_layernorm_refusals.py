@@ -29,3 +29,20 @@ def test_c_refusals():
         args = list(ok)
         args[at] = bad
         assert b(*args) == -1, (at, bad)
+
+
+def test_workgroups_cover_the_rows_as_the_kernel_takes_them():
+    """Backward's workgroups take four rows a group of lanes, up to 1024 x 256 lanes in all: 8 .. 64 lanes a row while 16 elements a lane
+    hold it (a multiple of 16 bytes each), then workgroups of 128 .. 1024 lanes.  A grid for fewer lanes a row than the kernel uses leaves
+    half of it to a second pass over the rows."""
+    from madiff_amd import lib
+    n = lib._lib.madiff_layer_norm_groups
+    for dt, per in ((1, 8), (0, 4)):
+        for C in list(range(1, 1100)) + [2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 32768]:
+            v = -(-C // per)
+            lanes = next((k for k in (8, 16, 32, 64) if v <= k), None) or next(k for k in (64, 128, 256, 512, 1024, 2048) if v <= k * 16 // per)
+            lanes = min(lanes, 1024)
+            block, rows_a_group = max(lanes, 256) if lanes <= 64 else lanes, 256 // lanes if lanes <= 64 else 1
+            for rows in (1, 64, 1000, 10 ** 7):
+                want = max(1, min(-(-rows // (4 * rows_a_group)), 1024 * 256 // block))
+                assert n(dt, rows, C) == want, (dt, rows, C, n(dt, rows, C), want)
