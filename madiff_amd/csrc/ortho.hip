@@ -504,8 +504,9 @@ struct NsFinish {
       for (int p = 0; p < 2; p++)
 #pragma unroll
         for (int r = 0; r < 8; r++) {
-          v[p][r] += c1 * ns_join(x.h1[p][r], x.l1[p][r]);
-          if (KIND == NS_SQUARE && e2) v[p][r] += q.c2 * ns_join(x.h2[p][r], x.l2[p][r]);
+          // (said, not left to the compiler, which took one or the other product for the exact one, by tile shape)
+          v[p][r] = fmaf(c1, ns_join(x.h1[p][r], x.l1[p][r]), v[p][r]);
+          if (KIND == NS_SQUARE && e2) v[p][r] = fmaf(q.c2, ns_join(x.h2[p][r], x.l2[p][r]), v[p][r]);
         }
     if constexpr (OUT == NS_OUT_PLANES) {
       // what no tile computes: the mirror images of tiles to the right of their row of the diagonal
@@ -1116,7 +1117,7 @@ static const int NS_SLOTS = 512;                              // two workgroups 
 static const int ns_lens[] = {1 << 30, 512, 320, 256, 192, 160, 128, 112, 96, 80, 64, 56, 48, 40, 32, 24, 16, 12, 8};
 
 // `batch` equal matrices
-static double ns_choose(int kind, int batch, int sp, int lp, int& shape, int& parts) {
+static void ns_choose(int kind, int batch, int sp, int lp, int& shape, int& parts) {
   const int ks = ns_ksteps(kind, sp, lp);
   double best = -1.0;
   for (int s = 0; s < 2; s++)
@@ -1128,10 +1129,14 @@ static double ns_choose(int kind, int batch, int sp, int lp, int& shape, int& pa
       const double t = rounds * ns_tile_time(ns_shapes[s], ks, p, n <= 256.0) + ns_join_time(ns_shapes[s], p, n);
       if (best < 0.0 || t < best) { best = t; shape = s; parts = p; }
     }
-  return best;
 }
 
-// one A and one pass over X saved against four square products more
+// Two steps in one: one A and one pass over X saved against four square products more.  For equal matrices it goes by their sides alone,
+// so that a matrix gets the same form alone, in a batch and in what is left of one.  Step by step and in twos, us: 12 x 333 x 1001 220
+// and 205, one of them 130 and 139; 12 x 1024 x 2048 1444 and 1303, one 254 and 255; 7 x 1024 x 5120 1927 and 1450; below twice as long
+// 24 x 333 x 500 241 and 244, one 118 and 131, 12 x 1024 x 1500 1183 and 1159, one 233 and 244.  A plan, whose launches hold all
+// its matrices, has one form for them all, by the time of its launches.
+static inline bool ns_pairs(int sp, int lp) { return lp >= 2 * sp; }
 static inline bool ns_pairs(const double (&time)[3]) { return time[NS_GRAM] + time[NS_APPLY] > 4.0 * time[NS_SQUARE]; }
 
 struct NsRun {                     // one call
@@ -1274,17 +1279,16 @@ static int ns_uniform(int batch, int rows, int cols, NsRun& r, long& ws_bytes) {
     return 0;
   }
   long slots = 0;
-  double time[3];
   for (int k = 0; k < 3; k++) {
     int parts = 1;
-    time[k] = ns_choose(k, batch, m.sp, m.lp, r.shape[k], parts);
+    ns_choose(k, batch, m.sp, m.lp, r.shape[k], parts);
     const int tiles = ns_tiles_of(k, r.shape[k], m.sp, m.lp);
     r.work[k] = {nullptr, batch * tiles * parts, tiles, parts};
     if (parts > 1 && r.work[k].n > r.grp.n_counters) r.grp.n_counters = r.work[k].n;
     const long bytes = parts > 1 ? (long)r.work[k].n * ns_shapes[r.shape[k]].bm * ns_shapes[r.shape[k]].bn * 4 : 0;
     slots = bytes > slots ? bytes : slots;
   }
-  r.pairs = ns_pairs(time);
+  r.pairs = ns_pairs(m.sp, m.lp);
   r.grp.counters = ws * batch + slots;
   ws_bytes = r.grp.counters + ((long)r.grp.n_counters * 4 + 255) / 256 * 256;
   return 0;

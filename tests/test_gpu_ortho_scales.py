@@ -142,3 +142,29 @@ def test_small_columns(rows, cols):
     bound = 5 * _rows(f32 - want) + (LAST + 2.0 ** -23) * _rows(want) + 7200 * math.sqrt(min(rows, cols)) * 2.0 ** -48
     off = _rows(got - want)
     assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(64, 128, 640), (64, 200, 600), (70, 600, 200)])
+def test_the_form_does_not_depend_on_the_batch(batch, rows, cols, monkeypatch):
+    """bf16 results may take two steps in one; whether they do goes by a matrix's own sides.  No reduction is cut at these sizes, so a
+    matrix has the same bits alone, in a batch, and in the shorter call at a batch's end."""
+    from madiff_amd import ops
+    x = torch.randn(batch, rows, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2)).bfloat16()
+    whole = ops.orthogonalize(x)
+    assert torch.equal(whole[5], ops.orthogonalize(x[5]))
+    monkeypatch.setattr(ops, "ORTHO_MAX_BATCH", batch - 1)
+    assert torch.equal(whole, ops.orthogonalize(x))
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_cut_reductions_in_batches(t):
+    """333 x 1001 is cut into 5, 4, 3 and 1 parts in batches of 1, 2, 4 and 12: other bits, the same bound (twice for two steps in one)."""
+    from madiff_amd import ops
+    x = torch.randn(12, 333, 1001, device=DEV, generator=torch.Generator(device=DEV).manual_seed(6)).to(t)
+    want, f32 = newton_schulz(x.double()), newton_schulz(x.float()).double()
+    n = lambda v: v.square().sum((-2, -1)).sqrt()                                                    # noqa: E731
+    last, times = (2.0 ** -23, 1) if t == torch.float32 else (2.0 ** -8, 2)
+    bound = times * (5 * n(f32 - want) + LAST * n(want)) + last * n(want)
+    for batch in (1, 2, 4, 12):
+        got = torch.cat([ops.orthogonalize(p) for p in x.split(batch)]).double()
+        assert bool((n(got - want) <= bound).all()), (batch, float((n(got - want) / bound).max()))
