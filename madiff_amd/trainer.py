@@ -62,13 +62,17 @@ class FlatAdamEMA:
         # on the "wgrad" auxiliary stream; data parallel: on the communication stream right behind the bucket's
         # all-reduce), so the HBM-bound Adam/EMA pass runs under the MFMA-bound rest of backward instead of after it
         self.overlap = os.environ.get("MADIFF_OVERLAP_ADAM", "1") != "0"
-        self.graphable = True            # may GraphedTrainStep capture steps of this optimizer?
         self._announced = None           # (do_ema, device_state) of the step whose backward is running (begin_step)
         self._main_stream = None
         # data-parallel capture: put the bucket event nodes on the MAIN branch, i.e. rejoin the parallel branches into it
         # at every bucket (a serialisation point per bucket; default off.  Kept as a tested alternative topology, see
         # DESIGN.md section 5 "capture failures")
         self.bucket_events_on_main = os.environ.get("MADIFF_BUCKET_EVENTS_ON_MAIN") == "1"
+
+    @property
+    def graphable(self) -> bool:
+        """May GraphedTrainStep capture steps of this optimizer?"""
+        return True
 
     # ------------------------------------------------------------------ setup after the first backward
     def _materialise(self):
@@ -493,12 +497,15 @@ class FlatMuonEMA(FlatAdamEMA):
         ops._check_newton_schulz("FlatMuonEMA", ns_steps, ops.NEWTON_SCHULZ, 1e-7)
         self.momentum, self.nesterov, self.weight_decay, self.ns_steps, self.select = momentum, nesterov, weight_decay, ns_steps, select
         self.overlap = False
-        # a captured step of this optimizer next to a live process group has ended the process once, in hipStreamEndCapture, by an
-        # abort of a thread of the group's whose cause is not known: data-parallel steps are issued eagerly
-        self.graphable = not self.dp
         self.plan: Optional[MuonPlan] = None
         self.matrices: List[str] = []              # their names
         self.split = 0                             # first element of the matrices
+
+    @property
+    def graphable(self) -> bool:
+        """Not next to a live process group, of one rank or many: the end of such a capture has ended the process once, by an abort
+        in a thread that is not Python's, and its cause is not known.  Steps are issued eagerly there."""
+        return not (dist.is_available() and dist.is_initialized())
 
     def _layout_order(self, order, name_of, known):
         embedded = {id(m.weight) for m in self.module.modules() if isinstance(m, torch.nn.Embedding)}
@@ -662,7 +669,7 @@ class GraphedTrainStep:
         capture stream (allocator / autograd warm-up), with EMA mode warm_do_ema; its (loss, infos) is `self.first`."""
         assert opt.flat_p is not None and opt.use_hip
         if not opt.graphable:
-            raise NotImplementedError(f"{type(opt).__name__}: data-parallel steps are issued eagerly (train_step), not captured")
+            raise NotImplementedError(f"{type(opt).__name__}: steps next to a process group are issued eagerly (train_step), not captured")
         self._warm_ema = int(warm_do_ema)
         self.dp = opt.dp
         self.single = isinstance(example_batch, dict)

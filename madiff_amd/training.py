@@ -155,7 +155,13 @@ class Trainer(object):
         self.rank = dist.get_rank() if self.world > 1 else 0
         self.dataset = dataset
         on_gpu = torch.device(train_device).type == "cuda"
-        self.use_graph = on_gpu if use_graph is None else use_graph
+        # Adam(lr, torch defaults) + EMA over the same parameters as the reference's torch.optim.Adam (training.py:109)
+        self.optimizer = OPTIMIZERS[optimizer](diffusion_model, self.ema_model, lr=train_lr, ema_decay=ema_decay,
+                                               bucket_mb=bucket_mb, **(optimizer_kwargs or {}))
+        if use_graph and not self.optimizer.graphable:
+            raise NotImplementedError(f"Trainer: use_graph with optimizer={optimizer!r} next to a process group (its steps are issued "
+                                      "eagerly; leave use_graph at None)")
+        self.use_graph = (on_gpu if use_graph is None else use_graph) and self.optimizer.graphable
         # a failed capture of the train step raises unless this is set (then all ranks drop to the eager step together)
         self.allow_eager_fallback = (os.environ.get("MADIFF_ALLOW_EAGER_FALLBACK") == "1"
                                      if allow_eager_fallback is None else bool(allow_eager_fallback))
@@ -170,13 +176,6 @@ class Trainer(object):
             self.dataloader_vis = cycle(torch.utils.data.DataLoader(
                 self.dataset, batch_size=1, num_workers=0, shuffle=True, pin_memory=on_gpu))
         self.renderer = renderer
-        # Adam(lr, torch defaults) + EMA over the same parameters as the reference's torch.optim.Adam (training.py:109)
-        self.optimizer = OPTIMIZERS[optimizer](diffusion_model, self.ema_model, lr=train_lr, ema_decay=ema_decay,
-                                               bucket_mb=bucket_mb, **(optimizer_kwargs or {}))
-        if use_graph and not self.optimizer.graphable:
-            raise NotImplementedError(f"Trainer: use_graph with optimizer={optimizer!r} under data parallelism (its steps are issued "
-                                      "eagerly; leave use_graph at None)")
-        self.use_graph = self.use_graph and self.optimizer.graphable
         self.optimizer.broadcast_parameters(0)
         self.bucket = bucket
         self.n_reference = n_reference

@@ -226,3 +226,25 @@ def test_gradients_below_eps():
         want = -lr * 0.2 * math.sqrt(18) * x
         got = net.conv.weight.detach().double().reshape(8, 18)
         assert float((got - want).norm()) <= 0.007 * float(want.norm()), size
+
+
+def test_no_capture_next_to_a_process_group(monkeypatch):
+    """The end of a capture next to a live process group is what once ended the process: a Muon step is not captured there, be the
+    group of one rank and its gradients not reduced, and be it there from the start or since.  Adam's, older and tested, is."""
+    import torch.distributed as dist
+    from diffuser.utils import Trainer
+    from madiff_amd.trainer import FlatAdamEMA, FlatMuonEMA
+    monkeypatch.delenv("MADIFF_FORCE_DP", raising=False)
+    before = FlatMuonEMA(_net(), None)
+    assert before.graphable and FlatAdamEMA(_net(), None).graphable
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{29300 + os.getpid() % 400}", rank=0, world_size=1)
+    try:
+        opt = FlatMuonEMA(_net(), None)
+        assert not opt.dp and not opt.graphable and not before.graphable
+        assert FlatAdamEMA(_net(), None).graphable
+        with pytest.raises(NotImplementedError):
+            Trainer(_net(), None, None, train_device="cpu", optimizer="muon", use_graph=True)
+        assert not Trainer(_net(), None, None, train_device="cpu", optimizer="muon").use_graph
+    finally:
+        dist.destroy_process_group()
+    assert before.graphable
