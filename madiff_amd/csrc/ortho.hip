@@ -752,7 +752,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
     // adds them up in part order (the same bits whoever it is) and goes on; nobody waits.  Sums and counter go past the XCDs' own
     // L2s (agent-scope accesses; the stores have arrived before the count).  Fences instead write back and drop whole L2s: 1300 us
     // where this takes 734 (2048 x 2048).  The sum as a launch of its own: a Muon step of 75 small matrices 150 us, so 131; 256 x
-    // 2048 144, so 124; 1024 x 5120 421, so 416; only squares lose, 2048 x 2048 had 684 (a tile's sums all go to one workgroup).
+    // 2048 144, so 124; 1024 x 5120 421, so 416; only squares lose, 2048 x 2048 had 684 (a tile's sums all go to one workgroup).  (All
+    // of that while hi and lo products shared a sum; now, in the same order, 743, 126, 130, 434.)
     float* to = (float*)(grp.ws + grp.partials) + (size_t)t.slot * (BM * BN) + (size_t)wave * (TI * TJ * 1024) + lane * 2;
     int* counter = (int*)(grp.ws + grp.counters) + t.slot;
     ns_unroll<TI * TJ>([&](auto at) __attribute__((always_inline)) {
@@ -807,13 +808,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
 }
 
 // ------------------------------------------------------------------------------------------------ one workgroup a matrix
-// A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything: by launches
-// a 16 x 128 matrix takes 84 us, next to none of it work; here 18 (64 x 512: 69, 128 x 96: 51; by launches 84 to 92).
+// A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything, of 19 us for a
+// 16 x 128 matrix (64 x 512: 68, 128 x 96: 52); its seventeen launches took 84, next to none of it work.
 // What bounds it is one CU's chain of dependent products, fifteen of them with a barrier or two each.  NW waves deal the
 // 32 x 32 blocks of a product among them (no mirror images: the whole squares are computed); a product that overwrites what it
 // reads keeps its blocks in registers until everybody has read.
-// Eight waves up to 64 rows, sixteen (which spill) above: a thousand of 16 x 128 53 us (with sixteen 81, with four 60), of 64 x 512
-// 335 (409), one 128 x 128 71 with sixteen and 81 with eight; a thousand of 128 x 160 the other way round, 389 and 351.
+// Eight waves up to 64 rows, sixteen (which spill) above, us a call in a row of calls: a thousand of 16 x 128 46 (with sixteen 77), of
+// 64 x 512 305 (383), one 128 x 160 69 with sixteen and 75 with eight; a thousand of 128 x 160 the other way round, 398 and 312.
 #define NS_SMALL_LDS 163840
 #define NS_TINY_LDS 32768
 
@@ -1053,8 +1054,9 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
   }
 }
 
-// Whatever fits goes through LDS.  Both ways measured, fp32, a call at a time: one matrix 16 x 128 29 us (by launches 93),
-// 64 x 512 79 (101), 128 x 160 78 (100); a thousand 16 x 128 53 (189), 64 x 512 335 (628), 128 x 160 389 (692).
+// Whatever fits goes through LDS.  Both ways measured, fp32, single calls from an idle GPU (some 10 us of which are the way there): one
+// matrix 16 x 128 29 us (by launches 95), 64 x 512 78 (117), 128 x 160 77 (108); a thousand 16 x 128 53 (199), 64 x 512 321 (664),
+// 128 x 160 383 (766).
 static inline long ns_small_bytes(const NsMat& m) { return 4L * m.sp * m.lp + 4L * m.sp * m.sp; }
 static inline bool ns_small(const NsMat& m) { return m.sp <= 128 && ns_small_bytes(m) <= NS_SMALL_LDS - 128; }
 
