@@ -361,10 +361,11 @@ int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, lo
 
 /* Newton-Schulz orthogonalisation (no counterpart in the reference, whose optimizer is Adam): `batch` row-major matrices
  * [rows, cols], back to back in src and in dst (dst == src is allowed), `dtype` storage.  With X = G or its transpose, short side
- * first, over max(|G|_F, eps):  `steps` times  A = X X^T,  X <- a X + (b A + c A A) X.  Operands are kept as two fp16 numbers, 22 bits
- * for values of X, A and the polynomials in A down to 2^-25 and a step of 2^-47 below, and multiplied by three fp16 matrix
- * instructions; everything is summed in fp32, the norm in 64 bits: a row's error is an fp32 iteration's down to rows 1e-6 of
- * the largest, and grows in proportion for smaller ones.  A matrix below eps is carried through the steps at a power of two of its
+ * first, over max(|G|_F, eps):  `steps` times  A = X X^T,  X <- a X + (b A + c A A) X.  Up to 32 rows of X (of at most 1024 columns;
+ * 2048 up to 16 rows) everything is fp32.  Else operands are kept as two fp16 numbers, 22 bits for values of X, A and the polynomials
+ * in A down to 2^-25 and a step of 2^-47 below, and multiplied by three fp16 matrix instructions; everything is summed in fp32,
+ * the norm in 64 bits: a row's error is an fp32 iteration's down to rows 1e-6 of the largest, and grows in proportion for
+ * smaller ones.  A matrix below eps is carried through the steps at a power of two of its
  * own, so its size costs no bits.  rows, cols: the shorter up to 16384, the longer up to 2^22.  ws: madiff_ortho_ws() bytes, 256-byte aligned, used during the call only; calls that may
  * overlap need one each. */
 int madiff_ortho_ws(int batch, int rows, int cols, long* ws_bytes);

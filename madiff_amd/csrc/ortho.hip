@@ -12,7 +12,9 @@
 // coefficients; other coefficients are checked on the host).  Values keep their 22 bits down to 2^-25; what is smaller is held to a
 // step of 2^-47.  (The second sum is for that: with lo in hi's unit the bits went below 2^-13 already and the step was 2^-35.  Of a 200 x
 // 600 matrix whose other half of rows is 1e-6 times the first, small rows came out 2.4e-3 off, now 8e-7, an fp32 iteration's 2.7e-6.
-// It costs 128 x 128 tiles 34 registers; 7 x 1024 x 5120 took 1981 us and takes 1999, 5 x 2048 x 256 156 and 161, 16 x 128 18.2 and 18.7.)
+// It costs 128 x 128 tiles 34 registers; 7 x 1024 x 5120 took 1981 us and takes 1999, 5 x 2048 x 256 156 and 161.)  Against 64 bits the
+// result is nearer than an fp32 iteration's from 96 rows on (half as far off at 200) and 0.7 to 1.4 times as far off, by length and
+// spectrum, between 32 and 96; fewer rows than that go in fp32 (ns_rows_kernel) unless they are very long or in a plan.
 //
 // Storage: a matrix [R, K] (both padded with zeros to multiples of 32) is a grid of blocks of 16 rows x 16 columns, 1 KB each, a
 // row's blocks one after the other.  In a block every row has four 16-byte chunks: hi of columns 0-7, hi of 8-15, lo of 0-7, lo of
@@ -807,14 +809,178 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
   });
 }
 
+// ------------------------------------------------------------------------------------------------ up to 32 rows, in registers
+// At these sizes sums are short and the 22 bits of a split operand would show (1.1 to 1.8 times an fp32 iteration's error): fp32 matrix
+// instructions, and no operand leaves the registers.  A wave has blocks of 16 columns of X, each twice for every 16 rows: `down`, lane (q, n)
+// with X[4 q + r][n], and `along`, with X[n][4 q + r], r = 0 .. 3.  A 16 x 16 x 4 instruction takes L[n][q] and M[q][n] from lane (q, n) and
+// leaves D[4 q + r][n] there, so four of them over r multiply
+//     along by along:  the block's part of A = X X^T          A and R, which are symmetric, by themselves:  A A
+//     R by down:  R X as `down`                               down by R:  (R X)^T, which is R X as `along`
+// (where there are many blocks a wave turns R X in LDS instead of forming it twice).  The waves' parts of A meet in LDS and are added up in wave order: by everybody, one barrier a step, or, where that would be
+// more reading, block by block by one wave each.
+template <bool BF16, int RB, int NW, int U>                  // row blocks, waves, column blocks a wave
+__global__ __launch_bounds__(64 * NW) void ns_rows_kernel(const void* __restrict__ src, void* __restrict__ dst, NsMat one, long stride,
+                                                      int steps, float a, float b, float c, float eps) {
+  constexpr int Q = RB * RB;
+  constexpr bool TWICE = NW * Q > 8;
+  // TWICE: the parts, then the sums.  Else two sets of parts by turns: who writes a step's has seen everybody behind the last one's.
+  __shared__ f32x4 parts[NW > 1 ? (TWICE ? NW + 1 : 2 * NW) * Q * 64 : 1];
+  __shared__ double norms[NW];
+  constexpr bool TURN = RB > 1 || U > 4;
+  __shared__ float turns[TURN ? NW * 16 * 20 : 1];
+  const NsMat& M = one;
+  const long at0 = (long)blockIdx.x * stride;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, n = lane & 15;
+  auto value = [&](int row, int col) __attribute__((always_inline)) {          // of X; 0 outside
+    const long e = at0 + (M.tall ? (long)col * M.cols + row : (long)row * M.cols + col);
+    if (row >= M.s || col >= M.l) return 0.f;
+    return BF16 ? to_f32(((const bf16_t*)src)[e]) : ((const float*)src)[e];
+  };
+  f32x4 down[U][RB], along[U][RB];
+  double sum = 0.0;
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      const int col = 16 * (wave + NW * u);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        down[u][i][r] = value(16 * i + 4 * q + r, col + n);
+        along[u][i][r] = value(16 * i + n, col + 4 * q + r);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r++) sum += (double)down[u][i][r] * (double)down[u][i][r];
+      if constexpr (U > 4) __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if constexpr (NW > 1) {
+    if (lane == 0) norms[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) sum += norms[w];
+  }
+  const double norm = sqrt(sum), over = norm > (double)eps ? norm : (norm <= (double)eps ? (double)eps : norm);      // (NaN stays)
+  int two;
+  const float inv = (float)(1.0 / frexp(over, &two));        // over = 2^two / inv, whatever its size
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        down[u][i][r] = ldexpf(down[u][i][r], -two) * inv;
+        along[u][i][r] = ldexpf(along[u][i][r], -two) * inv;
+      }
+  auto multiply = [](const f32x4& x, const f32x4& y, f32x4& d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], d, 0, 0, 0);
+  };
+  const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+  for (int step = 0; step < steps; step++) {
+    f32x4 A[RB][RB], R[RB][RB];
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int j = 0; j < RB; j++) {
+        A[i][j] = none;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (16 * (wave + NW * u) < M.l) multiply(along[u][i], along[u][j], A[i][j]);
+      }
+    if constexpr (NW > 1) {
+      f32x4* const s = parts + (TWICE ? 0 : (step & 1) * NW * Q * 64) + lane;
+#pragma unroll
+      for (int k = 0; k < Q; k++) s[(wave * Q + k) * 64] = A[k / RB][k % RB];
+      __syncthreads();
+      if constexpr (TWICE) {
+        static_assert(Q <= NW, "a wave a block");
+        if (wave < Q) {
+          f32x4 d = s[wave * 64];
+#pragma unroll
+          for (int w = 1; w < NW; w++) d += s[(w * Q + wave) * 64];
+          s[(NW * Q + wave) * 64] = d;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < Q; k++) A[k / RB][k % RB] = s[(NW * Q + k) * 64];
+      } else {
+#pragma unroll
+        for (int k = 0; k < Q; k++) {
+          A[k / RB][k % RB] = s[k * 64];
+#pragma unroll
+          for (int w = 1; w < NW; w++) A[k / RB][k % RB] += s[(w * Q + k) * 64];
+        }
+      }
+    }
+    // block (i, j) as lanes hold it is also block (j, i) as an instruction's left side
+#pragma unroll
+    for (int i = 0; i < RB; i++)
+#pragma unroll
+      for (int j = 0; j < RB; j++) {
+        R[i][j] = none;
+#pragma unroll
+        for (int k = 0; k < RB; k++) multiply(A[k][i], A[k][j], R[i][j]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) R[i][j][r] = fmaf(c, R[i][j][r], b * A[i][j][r]);
+      }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (16 * (wave + NW * u) >= M.l) continue;
+      f32x4 x[RB], y[RB];
+#pragma unroll
+      for (int i = 0; i < RB; i++) {
+        x[i] = y[i] = none;
+#pragma unroll
+        for (int k = 0; k < RB; k++) {
+          multiply(R[k][i], down[u][k], x[i]);
+          if constexpr (!TURN) multiply(down[u][k], R[k][i], y[i]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RB; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          down[u][i][r] = fmaf(a, down[u][i][r], x[i][r]);
+          if constexpr (!TURN) along[u][i][r] = fmaf(a, along[u][i][r], y[i][r]);
+        }
+      if constexpr (TURN) {
+        float* const t = turns + wave * (16 * 20);
+#pragma unroll
+        for (int i = 0; i < RB; i++) {
+          *(f32x4*)(t + n * 20 + 4 * q) = down[u][i];
+#pragma unroll
+          for (int r = 0; r < 4; r++) along[u][i][r] = t[(4 * q + r) * 20 + n];
+        }
+      }
+    }
+  }
+  // four neighbours of a row of G's a lane
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int i = 0; i < RB; i++) {
+      const f32x4 v = M.tall ? down[u][i] : along[u][i];
+      const int col = 16 * (wave + NW * u), row = M.tall ? col + n : 16 * i + n, at = M.tall ? 16 * i + 4 * q : col + 4 * q;
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (row < M.rows && at + r < M.cols) {
+          const long e = at0 + (long)row * M.cols + at + r;
+          if constexpr (BF16) ((bf16_t*)dst)[e] = (bf16_t)v[r];
+          else ((float*)dst)[e] = v[r];
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ one workgroup a matrix
-// A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything, of 19 us for a
-// 16 x 128 matrix (64 x 512: 68, 128 x 96: 52); its seventeen launches took 84, next to none of it work.
+// A small matrix whole in LDS (X and one square of it, split and laid out as in memory), one launch for everything: 64 x 512 takes 68 us,
+// 128 x 96 52, and by launches 90 to 100, next to none of it work.
 // What bounds it is one CU's chain of dependent products, fifteen of them with a barrier or two each.  NW waves deal the
 // 32 x 32 blocks of a product among them (no mirror images: the whole squares are computed); a product that overwrites what it
 // reads keeps its blocks in registers until everybody has read.
-// Eight waves up to 64 rows, sixteen (which spill) above, us a call in a row of calls: a thousand of 16 x 128 46 (with sixteen 77), of
-// 64 x 512 305 (383), one 128 x 160 69 with sixteen and 75 with eight; a thousand of 128 x 160 the other way round, 398 and 312.
+// Eight waves up to 64 rows, sixteen (which spill) above, us a call in a row of calls: a thousand of 64 x 512 305 (with sixteen 383), one
+// 128 x 160 69 with sixteen and 75 with eight; a thousand of 128 x 160 the other way round, 398 and 312.
 #define NS_SMALL_LDS 163840
 #define NS_TINY_LDS 32768
 
@@ -1054,11 +1220,16 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
   }
 }
 
-// Whatever fits goes through LDS.  Both ways measured, fp32, single calls from an idle GPU (some 10 us of which are the way there): one
-// matrix 16 x 128 29 us (by launches 95), 64 x 512 78 (117), 128 x 160 77 (108); a thousand 16 x 128 53 (199), 64 x 512 321 (664),
-// 128 x 160 383 (766).
+// Whatever else fits goes through LDS.  Both ways measured, fp32, single calls from an idle GPU (some 10 us of which are the way there):
+// one matrix 64 x 512 78 us (by launches 117), 32 x 1216 79 (116), 128 x 160 77 (108); a thousand 64 x 512 321 (664), 128 x 160 383 (766).
 static inline long ns_small_bytes(const NsMat& m) { return 4L * m.sp * m.lp + 4L * m.sp * m.sp; }
-static inline bool ns_small(const NsMat& m) { return m.sp <= 128 && ns_small_bytes(m) <= NS_SMALL_LDS - 128; }
+// Up to 32 rows in registers, fp32.  Both ways measured, calls in a row, through LDS as split fp16 and here: one 16 x 16 17 us and 11, 16 x
+// 128 21 and 12, 16 x 2000 104 (by launches) and 58, 32 x 128 21 and 20, 32 x 512 45 and 46, 32 x 1000 64 and 83; a thousand 16 x 128 47 and 21,
+// 32 x 32 37 and 26, 32 x 512 177 and 152, 32 x 1000 262 and 360.  From 512 columns on it is the error that decides (1.2 times an
+// fp32 iteration's and 0.9), which a bf16 result does not show.
+static inline bool ns_rows(const NsMat& m) { return m.s <= 32 && m.l <= (m.s <= 16 ? 2048 : 1024); }
+static inline bool ns_rows(const NsMat& m, int dtype) { return ns_rows(m) && (m.s <= 16 || m.l <= 512 || dtype == MADIFF_F32); }
+static inline bool ns_small(const NsMat& m) { return ns_rows(m) || (m.sp <= 128 && ns_small_bytes(m) <= NS_SMALL_LDS - 128); }
 
 // ------------------------------------------------------------------------------------------------ host
 struct NsPlan {                    // start of a plan; matrices and lists follow
@@ -1317,11 +1488,28 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
   hipLaunchKernelGGL((ns_small_kernel<BYTES, BF16, NW>), dim3(batch), dim3(64 * NW), 0, stream, src, dst, m, r.grp.at_stride, steps, \
                      a, b, c, eps, shift)
 #define NS_ANY(BYTES, NW) do { if (dtype == MADIFF_BF16) NS_GO(BYTES, true, NW); else NS_GO(BYTES, false, NW); } while (0)
-    if (ns_small_bytes(m) <= NS_TINY_LDS) NS_ANY(NS_TINY_LDS, 8);           // several workgroups a CU
+#define NS_ROWS(BF16, RB, NW, U)                                                                                                      \
+  hipLaunchKernelGGL((ns_rows_kernel<BF16, RB, NW, U>), dim3(batch), dim3(64 * NW), 0, stream, src, dst, m, r.grp.at_stride, steps, a, b, c, \
+                     eps)
+#define NS_ANY_ROWS(RB, NW, U) do { if (dtype == MADIFF_BF16) NS_ROWS(true, RB, NW, U); else NS_ROWS(false, RB, NW, U); } while (0)
+    if (ns_rows(m, dtype) && m.s <= 16) {
+      if (m.l <= 32) NS_ANY_ROWS(1, 1, 2);
+      else if (m.l <= 128) NS_ANY_ROWS(1, 4, 2);
+      else if (m.l <= 512) NS_ANY_ROWS(1, 8, 4);
+      else NS_ANY_ROWS(1, 16, 8);
+    } else if (ns_rows(m, dtype)) {
+      if (m.l <= 64) NS_ANY_ROWS(2, 4, 1);
+      else if (m.l <= 128) NS_ANY_ROWS(2, 4, 2);
+      else if (m.l <= 256) NS_ANY_ROWS(2, 8, 2);
+      else if (m.l <= 512) NS_ANY_ROWS(2, 8, 4);
+      else NS_ROWS(false, 2, 8, 8);
+    } else if (ns_small_bytes(m) <= NS_TINY_LDS) NS_ANY(NS_TINY_LDS, 8);    // several workgroups a CU
     else if (m.sp <= 64) NS_ANY(NS_SMALL_LDS, 8);
     else NS_ANY(NS_SMALL_LDS, 16);
 #undef NS_ANY
 #undef NS_GO
+#undef NS_ANY_ROWS
+#undef NS_ROWS
     MADIFF_CHECK_LAUNCH();
     return 0;
   }

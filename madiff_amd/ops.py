@@ -1798,9 +1798,10 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
                   eps: float = 1e-7) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of x [..., rows, cols] (float32 or bfloat16): every matrix, over max(|x|_F, eps), goes
     `steps` times through  X <- a X + (b A + c A A) X,  A = X X^T on its shorter side; its singular values end up near 1.
-    Whatever x's type, products are as accurate as float32 ones for values down to 2^-25 (of |X|_F <= 1) and hold smaller ones to
-    a step of 2^-47: rows 1e-6 of the largest are as near as in a float32 iteration, smaller ones less in proportion.  For bfloat16
-    matrices at least twice as long as wide two steps share one A (1.3 to 1.8 times a float32 iteration's error, before the rounding
+    Whatever x's type, products are as accurate as float32 ones: float32 for matrices of up to 32 rows (or columns) and 1024 of the
+    other, else for values down to 2^-25 (of |X|_F <= 1), smaller ones held to a step of 2^-47: rows 1e-6 of the largest are as near
+    as in a float32 iteration, smaller ones less in proportion.  For bfloat16 matrices of more than 32 rows, at least twice as long
+    as wide, two steps may share one A (1.3 to 1.8 times a float32 iteration's error, before the rounding
     to bfloat16).  The same call gives the same bits; in another batch a matrix may get others (how large tiles are and where long
     reductions are cut goes by the number of matrices), within the same bounds.  Returns a new contiguous tensor of x's shape and
     type.  Not differentiable, in either mode: an update is orthogonalised outside autograd."""
