@@ -216,3 +216,28 @@ def test_few_rows_of_any_size(rows, cols):
         want, f32, got = want.mT, f32.mT, got.mT
     bound = 5 * _rows(f32 - want) + (LAST + 2.0 ** -23) * _rows(want)
     assert bool((_rows(got - want) <= bound).all()), float((_rows(got - want) / bound).max())
+
+
+@pytest.mark.parametrize("rows,cols", [(2, 30), (16, 40), (12, 1500), (30, 100), (600, 32), (20, 900)])
+def test_few_rows_zero_nan_and_infinity(rows, cols):
+    from madiff_amd import ops
+    x = torch.randn(6, rows, cols, device=DEV, generator=torch.Generator(device=DEV).manual_seed(9))
+    whole = ops.orthogonalize(x)
+    y = x.clone()
+    y[1] = 0
+    y[2, rows - 1, 7] = float("nan")
+    y[4, 0, cols - 1] = float("-inf")
+    y[5] *= 2.0 ** 90                                         # squares beyond fp32: the same bits, a power of two cancels
+    got = ops.orthogonalize(y)
+    assert torch.equal(got[[0, 3, 5]], whole[[0, 3, 5]]) and bool((got[1] == 0).all())
+    assert bool(torch.isnan(got[2]).all()) and bool(torch.isnan(got[4]).all())
+    assert not bool(ops.orthogonalize(torch.zeros_like(x), eps=1e-30).any())
+    inner = x.clone()                                         # in place through the C entry, as its comment allows
+    import ctypes
+    from madiff_amd import lib
+    need = ctypes.c_long()
+    lib.call("madiff_ortho_ws", 6, rows, cols, ctypes.byref(need))
+    assert need.value == 0
+    lib.call("madiff_orthogonalize", lib.F32, inner.data_ptr(), inner.data_ptr(), 6, rows, cols, 5, *ops.NEWTON_SCHULZ, 1e-7, None, 0,
+             torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(inner, whole)
