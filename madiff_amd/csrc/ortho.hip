@@ -816,9 +816,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ns_product_kernel(NsGroup grp
 // leaves D[4 q + r][n] there, so four of them over r multiply
 //     along by along:  the block's part of A = X X^T          A and R, which are symmetric, by themselves:  A A
 //     R by down:  R X as `down`                               down by R:  (R X)^T, which is R X as `along`
-// (where there are many blocks a wave turns R X in LDS instead of forming it twice).  The waves' parts of A meet in LDS and are added up in wave order: by everybody, one barrier a step, or, where that would be
-// more reading, block by block by one wave each.  The kernel takes 4.4 us for 16 x 16, 7.1 for 16 x 128 (18.7 as split fp16 in LDS), 16 for
-// 32 x 128, 44 for 32 x 512: a step's products follow from each other, and from 32 x 256 on the fp32 matrix rate of the one CU counts.
+// (where there are many blocks a wave turns R X in LDS instead of forming it twice).  The waves' parts of A meet in LDS and are added up
+// in wave order: by everybody, one barrier a step, or, where that would be more reading, block by block by one wave each.
+// The kernel takes 4.4 us for 16 x 16, 7.1 for 16 x 128 (18.7 as split fp16 in LDS), 16 for 32 x 128, 44 for 32 x 512: a step's products
+// follow from each other, and from 32 x 256 on the fp32 matrix rate of the one CU counts.
 template <bool BF16, int RB, int NW, int U>                  // row blocks, waves, column blocks a wave
 __global__ __launch_bounds__(64 * NW) void ns_rows_kernel(const void* __restrict__ src, void* __restrict__ dst, NsMat one, long stride,
                                                       int steps, float a, float b, float c, float eps) {
