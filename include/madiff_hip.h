@@ -365,9 +365,9 @@ int madiff_layer_norm_bwd(int dtype, const void* x, long ldx, const void* dy, lo
  * 2048 up to 16 rows) everything is fp32.  Else operands are kept as two fp16 numbers, 22 bits for values of X, A and the polynomials
  * in A down to 2^-25 and a step of 2^-47 below, and multiplied by three fp16 matrix instructions; everything is summed in fp32,
  * the norm in 64 bits: a row's error is an fp32 iteration's down to rows 1e-6 of the largest, and grows in proportion for
- * smaller ones.  A matrix below eps is carried through the steps at a power of two of its
- * own, so its size costs no bits.  rows, cols: the shorter up to 16384, the longer up to 2^22.  ws: madiff_ortho_ws() bytes, 256-byte aligned, used during the call only; calls that may
- * overlap need one each. */
+ * smaller ones.  A matrix below eps is carried through the steps at a power of two of its own, so its size costs no bits.  rows,
+ * cols: the shorter up to 16384, the longer up to 2^22, and batch * rows * cols up to 2^33 with both rounded up to multiples of 64.  ws:
+ * madiff_ortho_ws() bytes, 256-byte aligned, used during the call only; calls that may overlap need one each. */
 int madiff_ortho_ws(int batch, int rows, int cols, long* ws_bytes);
 /* 0 when the steps of x <- x (a + b x^2 + c x^4) keep every start in [0, 1] inside what the products' operands hold (|values|
  * < 15), steps is in 1..64 and eps in [1e-30, 1e30); -1 otherwise, and then madiff_orthogonalize / madiff_muon_step refuse the call. */

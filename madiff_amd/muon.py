@@ -49,7 +49,8 @@ class MuonPlan:
         sc = (C.c_float * n)(*[1.0 if scales is None else float(v) for v in (scales or [1.0] * n)])
         need = C.c_long()
         if lib._lib.madiff_muon_plan(n, at, rows, cols, sc, None, 0, C.byref(need)) != 0:
-            raise ValueError("MuonPlan: a matrix is out of range (shorter side up to 16384, longer up to 4194304)")
+            raise ValueError("MuonPlan: a matrix is out of range (shorter side up to 16384, longer up to 4194304), or all of them have "
+                             "more than 2^33 elements")
         self._host = torch.zeros(need.value, dtype=torch.uint8)
         lib.call("madiff_muon_plan", n, at, rows, cols, sc, self._host.data_ptr(), need.value, C.byref(need))
         ws, elements = C.c_long(), C.c_long()

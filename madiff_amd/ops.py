@@ -1824,7 +1824,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Sequence[float]
     need = ctypes.c_long()
     if lib._lib.madiff_ortho_ws(1, rows, cols, ctypes.byref(need)) != 0:
         raise ValueError(f"orthogonalize: matrices of {rows} x {cols} are out of range (shorter side up to 16384, longer up to "
-                         "4194304)")
+                         "4194304, 2^33 elements)")
     dt, es = (lib.BF16 if x.dtype == torch.bfloat16 else lib.F32), x.element_size()
     most = max(1, min(batch, ORTHO_WS_BYTES // max(need.value, 1), ORTHO_MAX_BATCH))          # matrices a call
     while lib._lib.madiff_ortho_ws(most, rows, cols, ctypes.byref(need)) != 0:
