@@ -1227,7 +1227,7 @@ __global__ __launch_bounds__(64 * NW) void ns_small_kernel(const void* __restric
 static inline long ns_small_bytes(const NsMat& m) { return 4L * m.sp * m.lp + 4L * m.sp * m.sp; }
 // Up to 32 rows in registers, fp32.  Both ways measured, calls in a row, through LDS as split fp16 and here: one 16 x 16 17 us and 11, 16 x
 // 128 21 and 12, 16 x 2000 104 (by launches) and 58, 32 x 128 21 and 20, 32 x 512 45 and 46, 32 x 1000 64 and 83; a thousand 16 x 128 47 and 21,
-// 32 x 32 37 and 26, 32 x 512 177 and 152, 32 x 1000 262 and 360.  From 512 columns on it is the error that decides (1.2 times an
+// 32 x 32 37 and 26, 32 x 224 63 and 80, 32 x 256 122 and 82, 32 x 512 177 and 152, 32 x 1000 262 and 360.  From 512 columns on it is the error that decides (1.2 times an
 // fp32 iteration's and 0.9), which a bf16 result does not show.
 static inline bool ns_rows(const NsMat& m) { return m.s <= 32 && m.l <= (m.s <= 16 ? 2048 : 1024); }
 static inline bool ns_rows(const NsMat& m, int dtype) { return ns_rows(m) && (m.s <= 16 || m.l <= 512 || dtype == MADIFF_F32); }
@@ -1502,7 +1502,7 @@ extern "C" int madiff_orthogonalize(int dtype, const void* src, void* dst, int b
     } else if (ns_rows(m, dtype)) {
       if (m.l <= 64) NS_ANY_ROWS(2, 4, 1);
       else if (m.l <= 128) NS_ANY_ROWS(2, 4, 2);
-      else if (m.l <= 256) NS_ANY_ROWS(2, 8, 2);
+      else if (m.l <= 256) NS_ANY_ROWS(2, 4, 4);
       else if (m.l <= 512) NS_ANY_ROWS(2, 8, 4);
       else NS_ROWS(false, 2, 8, 8);
     } else if (ns_small_bytes(m) <= NS_TINY_LDS) NS_ANY(NS_TINY_LDS, 8);    // several workgroups a CU
